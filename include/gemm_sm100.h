@@ -50,7 +50,8 @@ enum { GS_OP_N = 0, GS_OP_T = 1, GS_OP_C = 2 };
 
 /* cudaDataType values (src/gemm.zig:14-49); the ones this backend computes on. */
 enum {
-    GS_R_32F = 0, GS_R_64F = 1, GS_R_16F = 2, GS_R_8I = 3, GS_R_32I = 10, GS_R_16BF = 14
+    GS_R_32F = 0, GS_R_64F = 1, GS_R_16F = 2, GS_R_8I = 3, GS_R_32I = 10, GS_R_16BF = 14,
+    GS_R_8F_E4M3 = 28, GS_R_8F_E5M2 = 29 /* the block-scaled FP8 calls below */
 };
 
 /* cublasComputeType_t values (src/gemm.zig:53-67). */
@@ -101,7 +102,8 @@ uint32_t gs_last_kernels(gs_handle handle);
 uint64_t gs_launch_count(gs_handle handle);
 /* Synchronises the handle's stream and returns the device error word that the
  * kernels' bounded waits write (0 = no error; bit 0 = a pipeline wait timed
- * out, bits 8..15 = where). The word is sticky for the handle's lifetime. */
+ * out, bits 8..15 = where; bit 1 = a gs_gemm_fp8_grouped call left out a group
+ * whose offsets were not multiples of 128). The word is sticky for the handle's lifetime. */
 gs_status gs_device_error(gs_handle handle, uint32_t *word);
 /* Limit, in SM clock cycles, of every bounded wait inside this handle's
  * tensor-core kernels (default 4e9, about 2 s at the B200's top clock; a value
@@ -129,7 +131,11 @@ enum {
     GS_KERNEL_TMAP = 1u << 6,     /* device-side tensor-map builder (pointer-array batches above
                                      GS_PTR_MAPS_IN_KERNEL_MAX_BATCH entries) */
     GS_KERNEL_TC_TF32 = 1u << 7,  /* COMPUTE_32F_FAST_TF32: operand split + tcgen05 kind::tf32 */
-    GS_KERNEL_REDUCE = 1u << 8    /* split-K: sum of the tensor-core kernel's per-slice partials, alpha/beta */
+    GS_KERNEL_REDUCE = 1u << 8,   /* split-K: sum of the tensor-core kernel's per-slice partials, alpha/beta */
+    GS_KERNEL_TC_F8 = 1u << 9,    /* block-scaled FP8 product, tcgen05 kind::f8f6f4 */
+    GS_KERNEL_QUANTIZE = 1u << 10, /* cast to block-scaled FP8 */
+    GS_KERNEL_ROUTE = 1u << 11,   /* expert choice, row plan, or their gradient */
+    GS_KERNEL_COMBINE = 1u << 12  /* experts' rows summed to tokens, or the gradient */
 };
 
 /* ---------------------------------------------------------------------- */
@@ -253,6 +259,165 @@ gs_status gs_gemm_batched_ex_noalloc(void *stream, int transa, int transb, int m
  * call on the device clears it. No counterpart in the reference; allocates
  * nothing. */
 gs_status gs_noalloc_device_error(void *stream, uint32_t *word);
+
+/* ---------------------------------------------------------------------- */
+/* Block-scaled FP8 products                                               */
+/* ---------------------------------------------------------------------- */
+/* No reference counterpart (slang-gemm has no 8-bit float type). An operand is
+ * a column-major matrix of FP8 bytes with f32 scales, one per 128 elements:
+ *  - GS_SCALE_VEC128: one per index i of the non-K axis and per 128 of K. The
+ *    scale of (i, K block b) is scale[i + b*lds] -- the non-K axis first,
+ *    whatever the operand's op.
+ *  - GS_SCALE_BLK128: one per 128 x 128 block, laid out as the operand is
+ *    stored: block (r/128, c/128) of the stored matrix has scale
+ *    scale[r/128 + (c/128)*lds]. One quantised weight therefore serves the
+ *    forward product (op T) and the input gradient (op N).
+ * A value is its FP8 number times its scale. The last block of an axis may be
+ * partial. The three products of a linear layer with row-major X [tokens, in],
+ * W [out, in], Y [tokens, out] are, column-major,
+ *   Y : m = out, n = tokens, k = in,     A = W  op T BLK128, B = X  op N VEC128
+ *   dX: m = in,  n = tokens, k = out,    A = W  op N BLK128, B = dY op N VEC128
+ *   dW: m = in,  n = out,    k = tokens, A = X  op N VEC128, B = dY op T VEC128
+ * where the operands of dW are quantised in vectors along the tokens (axis 1).
+ *
+ * These calls, as the others, are asynchronous on the handle's stream. They
+ * make the handle's device current for the call, so the caller's current
+ * device does not matter; they allocate nothing and keep no workspace in the
+ * handle, so graphs captured from one handle may run at the same time. */
+enum { GS_SCALE_VEC128 = 4, GS_SCALE_BLK128 = 5 }; /* cublasLtMatmulMatrixScale_t VEC128_32F, BLK128x128_32F */
+
+/* Casts a rows x cols column-major matrix of R_32F, R_16F or R_16BF to FP8
+ * (R_8F_E4M3 or R_8F_E5M2) with scales that are powers of two:
+ *   scale = the smallest 2^e >= 2^-126 with amax / 2^e <= the type's largest
+ *           value, amax over the block's finite elements (1 if amax is 0)
+ *   dst   = src / scale, rounded to nearest even
+ * NaN stays NaN; an infinity becomes NaN in E4M3 and stays one in E5M2.
+ * scaleMode GS_SCALE_VEC128: vectors of 128 down each column (axis 0; scale of
+ * (column c, rows 128b..) at scale[c + b*ldscale]) or along each row (axis 1;
+ * scale of (row r, columns 128b..) at scale[r + b*ldscale]). GS_SCALE_BLK128
+ * (axis 0): 128 x 128 blocks, scale[r/128 + (c/128)*ldscale].
+ * index: NULL, or cols int32 device values: column c is then read from source
+ * column index[c] / indexDiv of srcCols; a negative index, or one past the
+ * end, gives a column of zeros. With gs_moe_route's row_slot and indexDiv =
+ * top_k the cast puts the tokens in expert order. src and dst must not overlap. */
+gs_status gs_fp8_quantize(gs_handle handle, int scaleMode, int axis, int rows, int cols, const void *src, int srcType,
+                          int ldsrc, const int32_t *index, int indexDiv, int srcCols, void *dst, int dstType, int lddst,
+                          float *scale, int ldscale);
+
+/* C = alpha * op(A) * op(B) + beta * C over block-scaled FP8 operands; Atype
+ * and Btype may differ; C is R_32F, R_16F or R_16BF; alpha and beta are host
+ * floats. Each K block's 128 products are summed by the tensor core and added
+ * to f32 sums after scaling; C is rounded once. A and B must be 16-byte aligned
+ * with leading dimensions that are multiples of 16 (else
+ * GS_STATUS_NOT_SUPPORTED); m, n and k are free. */
+gs_status gs_gemm_fp8(gs_handle handle, int transa, int transb, int m, int n, int k, const float *alpha,
+                      const void *A, int Atype, int lda, const float *scaleA, int scaleModeA, int ldsa,
+                      const void *B, int Btype, int ldb, const float *scaleB, int scaleModeB, int ldsb,
+                      const float *beta, void *C, int Ctype, int ldc);
+
+/* The product over ragged groups, such as the experts of a routed layer:
+ * offsets holds groups + 1 int32 DEVICE values, group g covers
+ * [offsets[g], offsets[g+1]) of the ragged axis (an empty group is fine).
+ *  - GS_GROUP_N: columns of B and C are ragged; group g multiplies by its own
+ *    A + g*strideA with scales scaleA + g*strideScaleA (strideA a multiple of
+ *    16, 0 = one A for all). n is the column count of B and C; columns outside
+ *    every group are left as they are. op(B) must be N and B VEC128.
+ *  - GS_GROUP_K: K is ragged (weight gradients); group g writes its own
+ *    C + g*strideC, beta*C for an empty group. Each offset must be a multiple
+ *    of 128, except that groups may end at k: gs_moe_route aligns them. A group
+ *    that breaks this is not computed and sets bit 1 of the handle's device
+ *    error word. strideA and strideScaleA are ignored.
+ * strideC is ignored for GS_GROUP_N. Offsets outside [0, n] (or [0, k]) are
+ * clamped and decreasing ones raised, so no access leaves the operands.
+ * At most GS_FP8_MAX_GROUPS groups. */
+#define GS_FP8_MAX_GROUPS 1024
+enum { GS_GROUP_N = 0, GS_GROUP_K = 1 };
+gs_status gs_gemm_fp8_grouped(gs_handle handle, int ragged, int transa, int transb, int m, int n, int k, int groups,
+                              const int32_t *offsets, const float *alpha, const void *A, int Atype, int lda,
+                              long long strideA, const float *scaleA, int scaleModeA, int ldsa, long long strideScaleA,
+                              const void *B, int Btype, int ldb, const float *scaleB, int scaleModeB, int ldsb,
+                              const float *beta, void *C, int Ctype, int ldc, long long strideC);
+
+/* The tile a gs_gemm_fp8 (groups = 0) or gs_gemm_fp8_grouped call would use on
+ * a device with sm_count SMs: *columns per tile, *ctas (1 = 128 rows, 2 = a pair
+ * with 256) and *k_slices (CTAs of a cluster that share a tile's K). Pure host
+ * logic, for tests and capacity planning. */
+gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int k, int groups, int sm_count, int *columns,
+                           int *ctas, int *k_slices);
+
+/* ---------------------------------------------------------------------- */
+/* Routed experts around the grouped products                              */
+/* ---------------------------------------------------------------------- */
+enum { GS_ROUTE_SOFTMAX = 0, GS_ROUTE_SIGMOID = 1 };
+#define GS_ROUTE_MAX_EXPERTS 1024
+#define GS_ROUTE_MAX_TOP_K 32
+#define GS_ROUTE_MAX_GROUPS 32
+
+/* Routing of tokens to experts. For token t with logits l (tokens x experts,
+ * row t at logits + t*ld_logits; R_32F, R_16F or R_16BF):
+ *   s = softmax(l) over all experts, or sigmoid(l);  c = s + bias
+ *   of `groups` equal groups of consecutive experts, the `top_groups` with the
+ *   largest sum of their two largest c stay (ties: the lowest group)
+ *   the top_k largest c of those are chosen, in decreasing order (ties: the
+ *   lowest expert);  w = s of the chosen, divided by their sum if renormalize
+ *   (0 if the sum is 0), times scale
+ * Without a bias the order is the logits'. A logit of -inf or NaN masks its
+ * expert, as does a bias that makes c -inf or NaN; +inf counts as the largest
+ * finite logit. Where too few experts are left the last slots get id -1 and
+ * weight 0, and no row. The choice is the definition's in 64-bit arithmetic.
+ * token_count: NULL, or a device int32: tokens at and past it get ids -1.
+ * Plan (offsets != NULL): the rows of expert e are [offsets[e], offsets[e+1]),
+ * its slots t*top_k + j in increasing order, each expert's start rounded up to
+ * `align` rows (128 for GS_GROUP_K). slot_row[slot] is a slot's row or -1;
+ * row_slot[row] its slot, -1 for padding and for the rows behind the last
+ * expert's. rows (the length of row_slot) must be at least gs_moe_rows().
+ * workspace: at least gs_moe_route_workspace() bytes, 4-byte aligned, owned by
+ * the caller (one per call that may run at the same time). */
+typedef struct gs_route_desc {
+    int tokens, experts, top_k;
+    const void *logits; int logits_type; int ld_logits;
+    const float *bias;
+    int score, groups, top_groups, renormalize;
+    float scale;
+    const int32_t *token_count;
+    int align;
+    int32_t *ids;      /* tokens x top_k, token by token */
+    float *weights;    /* tokens x top_k */
+    int32_t *offsets;  /* experts + 1, or NULL */
+    int32_t *slot_row; /* tokens x top_k */
+    int32_t *row_slot; /* rows */
+    int rows;
+    void *workspace; size_t workspace_bytes;
+} gs_route_desc;
+
+gs_status gs_moe_route(gs_handle handle, const gs_route_desc *desc);
+/* Rows that a plan can need: tokens*top_k, and align - 1 more for every expert
+ * that can have one. Pure host logic. */
+gs_status gs_moe_rows(int tokens, int experts, int top_k, int align, int *rows);
+gs_status gs_moe_route_workspace(int tokens, int experts, int top_k, size_t *bytes);
+
+/* Gradient of the weights with respect to the logits, the choice held constant:
+ * reads desc's tokens, experts, top_k, logits, score, renormalize, scale and
+ * ids, and dweights (tokens x top_k); writes every element of dlogits (row t at
+ * dlogits + t*ld; of the logits' type or R_32F). Ids outside [0, experts) take
+ * no part. */
+gs_status gs_moe_route_backward(gs_handle handle, const gs_route_desc *desc, const float *dweights, void *dlogits,
+                                int dlogitsType, int lddlogits);
+
+/* out[t] = sum over j of weights[t, j] * y[slot_row[t, j]] in f32, in the order
+ * of j, rounded once; slots with row -1 (or outside [0, rows)) add nothing.
+ * Rows of y and out are hidden elements at y + r*ldy, out + t*ldout. weights
+ * NULL = 1, which makes it the gradient of the gather gs_fp8_quantize does. */
+gs_status gs_moe_combine(gs_handle handle, int tokens, int top_k, int hidden, const void *y, int yType, int ldy,
+                         int rows, const int32_t *slot_row, const float *weights, void *out, int outType, int ldout);
+
+/* Its gradient: dy[r] = weights[s] * dout[s / top_k] for the slot s = row_slot[r]
+ * (zeros for a row of no slot: every row of dy is written), dweights[s] =
+ * <dout[s / top_k], y[r]> in f32 (0 for a slot without a row). dout and dy have
+ * y's type. slot_row and row_slot are one plan's. */
+gs_status gs_moe_combine_backward(gs_handle handle, int tokens, int top_k, int hidden, const void *y, int yType, int ldy,
+                                  int rows, const int32_t *slot_row, const int32_t *row_slot, const float *weights,
+                                  const void *dout, int lddout, void *dy, int lddy, float *dweights);
 
 /* ---------------------------------------------------------------------- */
 /* Host-buffer mirror of gemm.gemmEx                                       */

@@ -1,0 +1,154 @@
+// moe_combine.cu -- sums the experts' rows back to their tokens, and the gradient.
+//
+//   out[t] = sum over j of w[t, j] * y[slot_row[t, j]]          (in order of j)
+//   dy[r]  = w[row_slot[r]] * dout[row_slot[r] / top_k]   (0 for a row of no slot)
+//   dw[t, j] = <dout[t], y[slot_row[t, j]]>
+//
+// Sums are f32 with one rounding at the end and a fixed order. Bound by memory:
+// 16-byte loads, all top_k rows of a token in flight at once.
+#include "gs_float.cuh"
+#include "gs_fp8.h"
+
+namespace gs {
+namespace combine {
+
+// Elements a thread handles at once: 16 bytes of the 16-bit types, 32 of f32.
+constexpr int V = 8;
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *p, int h, int hidden, float (&x)[V]) {
+    if (VEC && h + V <= hidden) {
+        const Pack<T, V> q = load_pack<T, V>(p + h);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = to_f32(q.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = h + i < hidden ? to_f32(p[h + i]) : 0.0f;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T *p, int h, int hidden, const float (&x)[V]) {
+    if (VEC && h + V <= hidden) {
+        Pack<T, V> q;
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.v[i] = from_f32<T>(x[i]);
+        store_pack<T, V>(p + h, q);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (h + i < hidden) p[h + i] = from_f32<T>(x[i]);
+    }
+}
+
+// A thread sums V columns of one token.
+template <typename T, typename TO, bool VEC>
+__global__ void __launch_bounds__(256) k_combine(const CombineDesc d) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int chunks = (d.hidden + V - 1) / V;
+    const long long tasks = static_cast<long long>(d.tokens) * chunks;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < tasks; i += static_cast<long long>(gridDim.x) * 256) {
+        const long long t = i / chunks;
+        const int h = static_cast<int>(i - t * chunks) * V;
+        float sum[V] = {};
+#pragma unroll 4
+        for (int j = 0; j < d.top_k; ++j) {
+            const long long at = t * d.top_k + j;
+            const int r = d.slot_row[at];
+            if (r < 0 || r >= d.rows) continue;
+            const float w = d.weights != nullptr ? d.weights[at] : 1.0f;
+            float x[V];
+            load8<T, VEC>(static_cast<const T *>(d.y) + r * d.ldy, h, d.hidden, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[v] = fmaf(w, x[v], sum[v]);
+        }
+        store8<TO, VEC>(static_cast<TO *>(d.out) + t * d.ldo, h, d.hidden, sum);
+    }
+}
+
+// A block handles one row of y: its dy, and its slot's weight gradient.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_combine_backward(const CombineDesc d) {
+    __shared__ float part[8];
+    grid_dep_wait();
+    grid_dep_launch();
+    const long long slots = static_cast<long long>(d.tokens) * d.top_k;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < slots; i += gridDim.x * 256LL) {
+        const int r = d.slot_row[i];
+        if (r < 0 || r >= d.rows) d.dweights[i] = 0.0f;  // a slot without a row
+    }
+    for (long long r = blockIdx.x; r < d.rows; r += gridDim.x) {
+        const int slot = d.row_slot[r];
+        T *dy = static_cast<T *>(d.dy) + r * d.lddy;
+        if (slot < 0 || slot >= slots) {
+            const float zero[V] = {};
+            for (int h = threadIdx.x * V; h < d.hidden; h += 256 * V) store8<T, VEC>(dy, h, d.hidden, zero);
+            continue;
+        }
+        const float w = d.weights[slot];
+        const T *y = static_cast<const T *>(d.y) + r * d.ldy;
+        const T *g = static_cast<const T *>(d.dout) + static_cast<long long>(slot / d.top_k) * d.lddo;
+        float dot = 0.0f;
+        for (int h = threadIdx.x * V; h < d.hidden; h += 256 * V) {
+            float a[V], b[V], o[V];
+            load8<T, VEC>(g, h, d.hidden, a);
+            load8<T, VEC>(y, h, d.hidden, b);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                dot = fmaf(a[v], b[v], dot);
+                o[v] = w * a[v];
+            }
+            store8<T, VEC>(dy, h, d.hidden, o);
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += part[k];
+            d.dweights[slot] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+static bool aligned(const void *p, long long ld, size_t es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * es) % 16 == 0; }
+
+}  // namespace combine
+
+cudaError_t launch_combine(Context &ctx, const CombineDesc &d) {
+    ctx.last_kernels |= GS_KERNEL_COMBINE;
+    const long long tasks = static_cast<long long>(d.tokens) * ((d.hidden + combine::V - 1) / combine::V);
+    const long long want = (tasks + 255) / 256, most = 32LL * ctx.sm_count;
+    const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
+    return with_float_type(d.type, [&](auto z) {
+        return with_float_type(d.out_type, [&](auto zo) {
+            using T = decltype(z);
+            using TO = decltype(zo);
+            const bool vec = combine::aligned(d.y, d.ldy, sizeof(T)) && combine::aligned(d.out, d.ldo, sizeof(TO));
+            const cudaError_t e = launch_pdl(vec ? combine::k_combine<T, TO, true> : combine::k_combine<T, TO, false>, dim3(blocks),
+                                             dim3(256), 0, ctx.stream, 1, d);
+            ctx.launches++;
+            return e;
+        });
+    });
+}
+
+cudaError_t launch_combine_backward(Context &ctx, const CombineDesc &d) {
+    ctx.last_kernels |= GS_KERNEL_COMBINE;
+    const long long most = 64LL * ctx.sm_count;
+    const unsigned blocks = static_cast<unsigned>(d.rows < 1 ? 1 : d.rows < most ? d.rows : most);
+    return with_float_type(d.type, [&](auto z) {
+        using T = decltype(z);
+        const bool vec = combine::aligned(d.y, d.ldy, sizeof(T)) && combine::aligned(d.dout, d.lddo, sizeof(T)) &&
+                         combine::aligned(d.dy, d.lddy, sizeof(T));
+        const cudaError_t e = launch_pdl(vec ? combine::k_combine_backward<T, true> : combine::k_combine_backward<T, false>, dim3(blocks),
+                                         dim3(256), 0, ctx.stream, 1, d);
+        ctx.launches++;
+        return e;
+    });
+}
+
+}  // namespace gs

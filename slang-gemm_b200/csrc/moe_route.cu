@@ -1,0 +1,508 @@
+// moe_route.cu -- routing of tokens to experts and the row plan of the grouped
+// products (gemm_fp8_sm100.cu) that follow, and the routing weights' gradient.
+//
+//   s = softmax(l) or sigmoid(l) over a token's logits l; c = s + bias
+//   the `top_groups` groups of experts with the largest sum of their two
+//   largest c stay; of their experts the `top_k` largest c are chosen, ties to
+//   the lowest index; w = scale * s (over the chosen ones' sum if renormalised)
+//
+// A logit of -inf or NaN (or a c of -inf or NaN) masks an expert: it is never
+// chosen, and a slot that finds no expert gets id -1 and weight 0. Without a bias
+// the experts' order is the logits' order, exactly. With one, or between groups,
+// c is computed in f32 and compared; where two values that decide something lie
+// closer than f32 can tell apart, the token is computed again in f64, so the
+// choice is that of the definition in 64 bits at f32's cost for nearly all
+// tokens.
+//
+// One warp per token, expert i * 32 + lane in register i. The plan is a stable
+// counting sort of the slots by expert (tokens in order, so nothing depends on
+// timing): counts per block of tokens, then every block sums the counts of the
+// blocks before it and ranks its own slots. Few slots take one block and one
+// launch.
+#include <type_traits>
+
+#include "gs_float.cuh"
+#include "gs_fp8.h"
+
+namespace gs {
+namespace route {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr uint32_t kFull = 0xffffffffu;
+
+// Order-preserving keys. -0 and 0 are one value.
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(double x) {
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x + 0.0));
+    return b ^ (static_cast<uint64_t>(static_cast<int64_t>(b) >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+    return __longlong_as_double(static_cast<long long>(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kFull, k); }
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+    const uint32_t hi = __reduce_max_sync(kFull, static_cast<uint32_t>(k >> 32));
+    const uint32_t lo = __reduce_max_sync(kFull, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+template <typename R>
+__device__ __forceinline__ R warp_sum(R v) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+    return v;
+}
+
+constexpr float kTop = 3.402823466e38f;  // +inf counts as the largest finite value
+
+// A token's logits, NaN and experts past the end as -inf.
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(const T *row, int experts, int lane, float (&l)[VPL]) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int e = i * 32 + lane;
+        float v = e < experts ? to_f32(row[e]) : -INFINITY;
+        if (!(v >= -INFINITY)) v = -INFINITY;
+        l[i] = fminf(v, kTop);
+    }
+}
+
+// Scores of all experts (masked ones: 0).
+template <typename R, int VPL>
+__device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, R (&s)[VPL]) {
+    if (sigmoid) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) s[i] = R(1) / (R(1) + exp_of(-R(l[i])));  // -inf: 1 / inf = 0
+        return;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
+    top = value_of(warp_max(key_of(top)));
+    R sum = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        s[i] = l[i] == -INFINITY ? R(0) : exp_of(R(l[i]) - R(top));
+        sum += s[i];
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s[i] = sum > R(0) ? s[i] / sum : R(0);
+}
+
+// Chooses a token's experts: lane j < top_k gets the j-th id and its score.
+// Returns false if f32 values that decide something are too close to call.
+template <typename R, int VPL>
+__device__ bool choose(const RouteDesc &d, const float (&l)[VPL], int lane, int &id, R &score) {
+    using Key = decltype(key_of(R(0)));
+    constexpr bool F32 = std::is_same<R, float>::value;
+    const Key none = key_of(R(-INFINITY));
+    R s[VPL];
+    scores<R, VPL>(l, d.sigmoid != 0, s);
+    Key key[VPL];
+    bool close = false;
+    // f32 error of a score, at most 1, and of its sum with the bias
+    auto far = [](float x, float y) { return !(fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x)); };
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        if (d.bias != nullptr) {
+            const int e = i * 32 + lane;
+            const R c = e < d.experts ? s[i] + R(d.bias[e]) : R(-INFINITY);
+            key[i] = l[i] == -INFINITY || !(c > R(-INFINITY)) ? none : key_of(c);
+        } else {
+            key[i] = key_of(R(l[i]));
+        }
+    }
+    if (d.groups > 1 && d.top_groups < d.groups) {
+        const int size = d.experts / d.groups;
+        const uint32_t magic = ((1u << 20) + static_cast<uint32_t>(size) - 1) / static_cast<uint32_t>(size);  // e / size, e and size <= 1024
+        Key mine = none;  // lane g: group g's score
+        for (int g = 0; g < d.groups; ++g) {
+            Key a1 = none, a2 = none;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const uint32_t e = static_cast<uint32_t>(i * 32 + lane);
+                Key k = none;
+                if (static_cast<int>((e * magic) >> 20) == g && key[i] != none) k = d.bias != nullptr ? key[i] : key_of(s[i]);
+                if (k > a1) { a2 = a1; a1 = k; }
+                else if (k > a2) a2 = k;
+            }
+            const Key m1 = warp_max(a1);
+            const int owner = __ffs(__ballot_sync(kFull, a1 == m1)) - 1;
+            const Key m2 = warp_max(lane == owner ? a2 : a1);
+            Key total = none;
+            if (m1 != none) total = key_of(value_of(m1) + (m2 != none ? value_of(m2) : R(0)));
+            if (lane == g) mine = total;
+        }
+        int better = 0;
+        for (int g = 0; g < d.groups; ++g) {
+            const Key other = __shfl_sync(kFull, mine, g);
+            better += other > mine || (other == mine && g < lane) ? 1 : 0;
+        }
+        const bool kept = lane < d.groups && better < d.top_groups;
+        if constexpr (F32) {
+            const Key worst = ~warp_max(kept ? ~mine : Key(0));
+            const Key best = warp_max(!kept && lane < d.groups ? mine : Key(0));
+            if (best > none && !far(value_of(worst), value_of(best))) close = true;
+        }
+        const uint32_t keep = __ballot_sync(kFull, kept);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const uint32_t g = (static_cast<uint32_t>(i * 32 + lane) * magic) >> 20;
+            if (g >= 32 || !((keep >> g) & 1u)) key[i] = none;
+        }
+    }
+    id = -1;
+    score = R(0);
+    Key last = none;
+    for (int j = 0; j <= d.top_k; ++j) {  // one more than chosen, for the distance to the first that is not
+        if (j == d.top_k && !(F32 && d.bias != nullptr)) break;
+        Key best = none;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (key[i] > best) { best = key[i]; at = i; }
+        const Key top = warp_max(best);
+        if (top == none) break;
+        if constexpr (F32) {
+            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(top))) close = true;
+        }
+        if (j == d.top_k) break;
+        last = top;
+        const uint32_t e = __reduce_min_sync(kFull, best == top ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
+        const int owner = static_cast<int>(e & 31u);
+        R v = R(0);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (lane == owner && i == static_cast<int>(e >> 5)) { v = s[i]; key[i] = none; }
+        v = __shfl_sync(kFull, v, owner);
+        if (lane == j) { id = static_cast<int>(e); score = v; }
+    }
+    return !close;
+}
+
+// Chooses and writes one token's ids and weights; returns lane j's id.
+template <typename T, int VPL>
+__device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, int lane) {
+    int id = -1;
+    float w = 0.0f;
+    if (t < live) {
+        float l[VPL];
+        load_row<T, VPL>(static_cast<const T *>(d.logits) + static_cast<long long>(t) * d.ld, d.experts, lane, l);
+        float s;
+        if (!choose<float, VPL>(d, l, lane, id, s)) {
+            double s64;
+            choose<double, VPL>(d, l, lane, id, s64);
+            s = static_cast<float>(s64);
+        }
+        w = s;
+        if (d.renorm) {
+            const float sum = warp_sum(w);
+            w = sum > 0.0f ? w / sum : 0.0f;
+        }
+        w *= d.scale;
+    }
+    if (lane < d.top_k) {
+        const long long at = static_cast<long long>(t) * d.top_k + lane;
+        d.ids[at] = id;
+        d.weights[at] = id < 0 ? 0.0f : w;
+    }
+    return id;
+}
+
+// Exclusive sums over the experts of their aligned counts: base[e] = first row of expert e, base[experts] = all rows.
+// Called by the whole block; `count` and `base` in shared memory.
+__device__ void expert_bases(const int *count, int *base, int experts, int align) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, per = (experts + 31) / 32;
+        const int lo = min(lane * per, experts), hi = min(lo + per, experts);
+        int sum = 0;
+        for (int e = lo; e < hi; ++e) sum += (count[e] + align - 1) / align * align;
+        int incl = sum;
+        for (int s = 1; s < 32; s <<= 1) {
+            const int v = __shfl_up_sync(kFull, incl, s);
+            if (lane >= s) incl += v;
+        }
+        int at = incl - sum;
+        for (int e = lo; e < hi; ++e) {
+            base[e] = at;
+            at += (count[e] + align - 1) / align * align;
+        }
+        if (lane == 31) base[experts] = incl;
+    }
+    __syncthreads();
+}
+
+// Rows of slots [lo, hi) of this block: next[w * experts + e] first counts warp w's slots of expert e, then becomes the
+// row of its next one. `first` gives each expert's first row for this block.
+__device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, long long hi, int *next, const int *first, int experts) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long per = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const long long a = min(lo + warp * per, hi), b = min(a + per, hi);
+    for (int i = threadIdx.x; i < kWarps * experts; i += kThreads) next[i] = 0;
+    __syncthreads();
+    for (long long i = a; i < b; i += 32) {
+        const int e = i + lane < b ? ids[i + lane - lo] : -1;
+        const uint32_t same = __match_any_sync(kFull, e);
+        if (e >= 0 && lane == __ffs(same) - 1) next[warp * experts + e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        int at = first[e];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const int n = next[w * experts + e];
+            next[w * experts + e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    for (long long i = a; i < b; i += 32) {
+        const int e = i + lane < b ? ids[i + lane - lo] : -1;
+        const uint32_t same = __match_any_sync(kFull, e);
+        int row = -1;
+        if (e >= 0) row = next[warp * experts + e] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (e >= 0 && lane == __ffs(same) - 1) next[warp * experts + e] += __popc(same);
+        __syncwarp();
+        if (i + lane < b) {
+            d.slot_row[i + lane] = row;
+            if (row >= 0 && row < d.rows) d.row_slot[row] = static_cast<int32_t>(i + lane);
+        }
+    }
+}
+
+// Rows that hold no slot: the padding behind an expert's rows, and the rows behind the last expert.
+__device__ void fill_padding(const RouteDesc &d, const int *count, const int *base, int block, int blocks) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (d.align > 1)
+        for (int e = block * kWarps + warp; e < d.experts; e += blocks * kWarps)
+            for (int r = base[e] + count[e] + lane; r < min(base[e + 1], d.rows); r += 32) d.row_slot[r] = -1;
+    for (long long r = base[d.experts] + static_cast<long long>(block) * kThreads + threadIdx.x; r < d.rows;
+         r += static_cast<long long>(blocks) * kThreads)
+        d.row_slot[r] = -1;
+}
+
+constexpr int kSmallSlots = 1024;
+
+// All in one block: few slots.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(kThreads) k_route_small(const RouteDesc d) {
+    extern __shared__ int sm[];
+    __shared__ int ids[kSmallSlots];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int live = d.token_count != nullptr ? *d.token_count : d.tokens;
+    for (int t = warp; t < d.tokens; t += kWarps) {
+        const int id = route_token<T, VPL>(d, t, live, lane);
+        if (lane < d.top_k) ids[t * d.top_k + lane] = id;
+    }
+    if (d.offsets == nullptr) return;
+    int *count = sm, *base = sm + d.experts, *next = base + d.experts + 1;
+    for (int e = threadIdx.x; e < d.experts; e += kThreads) count[e] = 0;
+    __syncthreads();
+    const int slots = d.tokens * d.top_k;
+    for (int i = threadIdx.x; i < slots; i += kThreads)
+        if (ids[i] >= 0) atomicAdd(&count[ids[i]], 1);  // whole numbers: any order gives the same sum
+    __syncthreads();
+    expert_bases(count, base, d.experts, d.align);
+    for (int e = threadIdx.x; e <= d.experts; e += kThreads) d.offsets[e] = base[e];
+    rank_slots(d, ids, 0, slots, next, base, d.experts);
+    fill_padding(d, count, base, 0, 1);
+}
+
+// Many slots, first kernel: the choice, and the block's count of every expert.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(kThreads) k_route_choose(const RouteDesc d, int per_block) {
+    extern __shared__ int sm[];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int live = d.token_count != nullptr ? *d.token_count : d.tokens;
+    const bool plan = d.offsets != nullptr;
+    if (plan) {
+        for (int e = threadIdx.x; e < d.experts; e += kThreads) sm[e] = 0;
+        __syncthreads();
+    }
+    const long long lo = static_cast<long long>(blockIdx.x) * per_block;
+    const int hi = static_cast<int>(min(lo + per_block, static_cast<long long>(d.tokens)));
+    for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += kWarps) {
+        const int id = route_token<T, VPL>(d, t, live, lane);
+        if (plan && id >= 0) atomicAdd(&sm[id], 1);
+    }
+    if (plan) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < d.experts; e += kThreads) d.hist[static_cast<long long>(blockIdx.x) * d.experts + e] = sm[e];
+    }
+}
+
+// Second kernel: every block sums the counts (all, and of the blocks before it), then ranks its slots.
+__global__ void __launch_bounds__(kThreads) k_route_plan(const RouteDesc d, int per_block) {
+    extern __shared__ int sm[];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int experts = d.experts;
+    int *count = sm, *before = count + experts, *base = before + experts, *next = base + experts + 1;
+    for (int i = threadIdx.x; i < 2 * experts; i += kThreads) sm[i] = 0;
+    __syncthreads();
+    const int parts = max(1, kThreads / experts), blocks = gridDim.x;
+    for (int i = threadIdx.x; i < experts * parts; i += kThreads) {
+        const int e = i % experts, part = i / experts;
+        int all = 0, mine = 0;
+#pragma unroll 8
+        for (int b = part; b < blocks; b += parts) {
+            const int n = d.hist[static_cast<long long>(b) * experts + e];
+            all += n;
+            if (b < static_cast<int>(blockIdx.x)) mine += n;
+        }
+        atomicAdd(&count[e], all);
+        atomicAdd(&before[e], mine);
+    }
+    __syncthreads();
+    expert_bases(count, base, experts, d.align);
+    if (blockIdx.x == 0)
+        for (int e = threadIdx.x; e <= experts; e += kThreads) d.offsets[e] = base[e];
+    for (int e = threadIdx.x; e < experts; e += kThreads) before[e] += base[e];
+    __syncthreads();
+    const long long slots = static_cast<long long>(d.tokens) * d.top_k;
+    const long long lo = min(static_cast<long long>(blockIdx.x) * per_block * d.top_k, slots);
+    const long long hi = min(lo + static_cast<long long>(per_block) * d.top_k, slots);
+    rank_slots(d, d.ids + lo, lo, hi, next, before, experts);
+    fill_padding(d, count, base, blockIdx.x, blocks);
+}
+
+template <typename T, int VPL>
+static cudaError_t launch(Context &ctx, const RouteDesc &d) {
+    const int blocks = route_blocks(d.tokens, d.top_k);
+    const size_t plan_ints = static_cast<size_t>(d.experts) * (kWarps + 3) + 1;
+    const size_t smem = plan_ints * sizeof(int);
+    if (smem > 40 * 1024) {  // with the static 4 KiB still within the 48 KiB that need no opt-in
+        cudaError_t e = cudaFuncSetAttribute(k_route_small<T, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(k_route_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    if (blocks == 0) {
+        const cudaError_t e = launch_pdl(k_route_small<T, VPL>, dim3(1), dim3(kThreads), smem, ctx.stream, 1, d);
+        ctx.launches++;
+        return e;
+    }
+    const int per = (d.tokens + blocks - 1) / blocks;
+    cudaError_t e = launch_pdl(k_route_choose<T, VPL>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
+                               static_cast<size_t>(d.experts) * sizeof(int), ctx.stream, 1, d, per);
+    ctx.launches++;
+    if (e != cudaSuccess || d.offsets == nullptr) return e;
+    e = launch_pdl(k_route_plan, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, ctx.stream, 1, d, per);
+    ctx.launches++;
+    return e;
+}
+
+// Gradient of the weights with respect to the logits; the choice is constant.
+//   softmax, renormalised: a softmax over the chosen experts alone
+//   otherwise dl = J^T ds, with ds_j = scale * (g_j - sum g w) / S or scale * g_j
+template <typename T, typename TD, int VPL>
+__global__ void __launch_bounds__(256) k_route_backward(const RouteBwdDesc d) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int lane = threadIdx.x & 31;
+    for (long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < d.tokens; t += static_cast<long long>(gridDim.x) * 8) {
+        float l[VPL], s[VPL];
+        load_row<T, VPL>(static_cast<const T *>(d.logits) + t * d.ld, d.experts, lane, l);
+        scores<float, VPL>(l, d.sigmoid != 0, s);
+        int id = -1;
+        float g = 0.0f;
+        if (lane < d.top_k) {
+            id = d.ids[t * d.top_k + lane];
+            if (id < 0 || id >= d.experts) id = -1;
+            else g = d.dweights[t * d.top_k + lane] * d.scale;
+        }
+        float sj = 0.0f, lj = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const float v = __shfl_sync(kFull, s[i], id & 31), x = __shfl_sync(kFull, l[i], id & 31);
+            if (id >= 0 && (id >> 5) == i) { sj = v; lj = x; }
+        }
+        // slope_j: what chosen expert j's own logit gets; common: what every logit gets, times its score (softmax)
+        float slope, common = 0.0f;
+        if (d.renorm) {
+            const float sum = warp_sum(sj);
+            const float w = sum > 0.0f ? sj / sum : 0.0f;
+            const float dev = g - warp_sum(g * w);
+            slope = id >= 0 ? w * dev : 0.0f;
+            if (d.sigmoid) slope *= 1.0f / (1.0f + expf(lj));
+        } else {
+            slope = g * sj;
+            if (d.sigmoid) slope *= 1.0f / (1.0f + expf(lj));
+            else common = warp_sum(slope);
+        }
+        float out[VPL];
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) out[i] = -common * s[i];
+        for (int j = 0; j < d.top_k; ++j) {
+            const int e = __shfl_sync(kFull, id, j);
+            const float v = __shfl_sync(kFull, slope, j);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (e >= 0 && e == i * 32 + lane) out[i] += v;
+        }
+        TD *row = static_cast<TD *>(d.dlogits) + t * d.ldd;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (i * 32 + lane < d.experts) row[i * 32 + lane] = from_f32<TD>(out[i]);
+    }
+}
+
+// Registers per lane for a number of experts (at most 1024).
+template <typename F>
+static cudaError_t with_vpl(int experts, F f) {
+    if (experts <= 32) return f(std::integral_constant<int, 1>{});
+    if (experts <= 64) return f(std::integral_constant<int, 2>{});
+    if (experts <= 128) return f(std::integral_constant<int, 4>{});
+    if (experts <= 256) return f(std::integral_constant<int, 8>{});
+    if (experts <= 512) return f(std::integral_constant<int, 16>{});
+    return f(std::integral_constant<int, 32>{});
+}
+
+}  // namespace route
+
+int route_blocks(int tokens, int top_k) {
+    if (static_cast<long long>(tokens) * top_k <= route::kSmallSlots) return 0;
+    const int by_tokens = (tokens + route::kWarps - 1) / route::kWarps;
+    return by_tokens < 148 ? by_tokens : 148;
+}
+
+cudaError_t launch_route(Context &ctx, const RouteDesc &d) {
+    ctx.last_kernels |= GS_KERNEL_ROUTE;
+    return with_float_type(d.type, [&](auto z) {
+        return route::with_vpl(d.experts, [&](auto v) { return route::launch<decltype(z), decltype(v)::value>(ctx, d); });
+    });
+}
+
+cudaError_t launch_route_backward(Context &ctx, const RouteBwdDesc &d) {
+    ctx.last_kernels |= GS_KERNEL_ROUTE;
+    const long long want = (static_cast<long long>(d.tokens) + 7) / 8, most = 8LL * ctx.sm_count;
+    const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
+    return with_float_type(d.type, [&](auto z) {
+        return route::with_vpl(d.experts, [&](auto v) {
+            using T = decltype(z);
+            // the gradient has the logits' type, or f32
+            auto kern = d.dtype == GS_R_32F ? route::k_route_backward<T, float, decltype(v)::value>
+                                            : route::k_route_backward<T, T, decltype(v)::value>;
+            const cudaError_t e = launch_pdl(kern, dim3(blocks), dim3(256), 0, ctx.stream, 1, d);
+            ctx.launches++;
+            return e;
+        });
+    });
+}
+
+}  // namespace gs

@@ -24,6 +24,7 @@ HEADER_PATH = os.path.join(_HERE, "..", "include", "gemm_sm100.h")
 # ---- enums (CUDA / cuBLAS integer values; src/gemm.zig:14-113) -------------
 OP_N, OP_T, OP_C = 0, 1, 2
 R_32F, R_64F, R_16F, R_8I, R_32I, R_16BF = 0, 1, 2, 3, 10, 14
+R_8F_E4M3, R_8F_E5M2 = 28, 29
 COMPUTE_16F, COMPUTE_16F_PEDANTIC = 64, 65
 COMPUTE_32F, COMPUTE_32F_PEDANTIC = 68, 69
 COMPUTE_32F_FAST_16F, COMPUTE_32F_FAST_16BF, COMPUTE_32F_FAST_TF32 = 74, 75, 77
@@ -50,8 +51,19 @@ KERNEL_SCALE = 1 << 5
 KERNEL_TMAP = 1 << 6
 KERNEL_REDUCE = 1 << 8
 KERNEL_TC_TF32 = 1 << 7
+KERNEL_TC_F8 = 1 << 9
+KERNEL_QUANTIZE = 1 << 10
+KERNEL_ROUTE = 1 << 11
+KERNEL_COMBINE = 1 << 12
 
 ELEM_SIZE = {R_32F: 4, R_64F: 8, R_16F: 2, R_8I: 1, R_32I: 4, R_16BF: 2}
+SCALE_VEC128, SCALE_BLK128 = 4, 5
+GROUP_N, GROUP_K = 0, 1
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+FP8_MAX_GROUPS = 1024       # GS_FP8_MAX_GROUPS
+ROUTE_MAX_EXPERTS = 1024    # GS_ROUTE_MAX_EXPERTS
+ROUTE_MAX_TOP_K = 32        # GS_ROUTE_MAX_TOP_K
+ROUTE_MAX_GROUPS = 32       # GS_ROUTE_MAX_GROUPS
 NOALLOC_MAX_BATCH = 256  # GS_NOALLOC_MAX_BATCH
 PTR_MAPS_IN_KERNEL_MAX_BATCH = 64  # GS_PTR_MAPS_IN_KERNEL_MAX_BATCH
 
@@ -102,6 +114,23 @@ class PtrBatchedDesc(ctypes.Structure):
     ]
 
 
+class RouteDesc(ctypes.Structure):
+    """gs_route_desc: the arguments of gs_moe_route and its gradient."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("top_k", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("logits_type", ctypes.c_int), ("ld_logits", ctypes.c_int),
+        ("bias", ctypes.c_void_p),
+        ("score", ctypes.c_int), ("groups", ctypes.c_int), ("top_groups", ctypes.c_int), ("renormalize", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("token_count", ctypes.c_void_p),
+        ("align", ctypes.c_int),
+        ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+        ("slot_row", ctypes.c_void_p), ("row_slot", ctypes.c_void_p), ("rows", ctypes.c_int),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -132,6 +161,17 @@ def _load() -> ctypes.CDLL:
         "gs_plan_gemm_strided_batched_ex": (st, [i, i, i, i, i, vp, i, i, ll, vp, i, i, ll, vp, i, i, ll, i, i,
                                                  ctypes.POINTER(u32)]),
         "gs_plan_tile": (st, [i, i, i, i, i, i, i, i, i, i, i, ctypes.POINTER(i), ctypes.POINTER(i)]),
+        "gs_fp8_quantize": (st, [vp, i, i, i, i, vp, i, i, vp, i, i, vp, i, i, vp, i]),
+        "gs_gemm_fp8": (st, [vp, i, i, i, i, i, vp, vp, i, i, vp, i, i, vp, i, i, vp, i, i, vp, vp, i, i]),
+        "gs_gemm_fp8_grouped": (st, [vp, i, i, i, i, i, i, i, vp, vp, vp, i, i, ll, vp, i, i, ll, vp, i, i, vp, i, i, vp,
+                                     vp, i, i, ll]),
+        "gs_plan_gemm_fp8": (st, [i, i, i, i, i, i, i, i, ctypes.POINTER(i), ctypes.POINTER(i), ctypes.POINTER(i)]),
+        "gs_moe_route": (st, [vp, ctypes.POINTER(RouteDesc)]),
+        "gs_moe_rows": (st, [i, i, i, i, ctypes.POINTER(i)]),
+        "gs_moe_route_workspace": (st, [i, i, i, ctypes.POINTER(ctypes.c_size_t)]),
+        "gs_moe_route_backward": (st, [vp, ctypes.POINTER(RouteDesc), vp, vp, i, i]),
+        "gs_moe_combine": (st, [vp, i, i, i, vp, i, i, i, vp, vp, vp, i, i]),
+        "gs_moe_combine_backward": (st, [vp, i, i, i, vp, i, i, i, vp, vp, vp, vp, i, vp, i, vp]),
         "gs_host_gemm_ex": (st, [vp, ctypes.POINTER(ExDesc)]),
         "gs_host_gemm_batched_ex": (st, [vp, ctypes.POINTER(PtrBatchedDesc)]),
         "gs_plan_shards": (st, [ll, i, ll, ctypes.POINTER(ll)]),
@@ -211,6 +251,32 @@ def plan_tile(transa, transb, m, n, k, atype, ctype, compute, batch=1, algo=GEMM
     s = _lib.gs_plan_tile(transa, transb, m, n, k, atype, ctype, compute, batch, algo, sm_count, ctypes.byref(tile),
                           ctypes.byref(parts))
     return s, tile.value, parts.value
+
+
+def plan_gemm_fp8(transa, transb, m, n, k, groups=0, ragged=GROUP_N, sm_count=148):
+    """gs_plan_gemm_fp8: (status, columns, ctas, k_slices) of the tile an FP8 product would use. Pure host logic."""
+    bn, cg, parts = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    s = _lib.gs_plan_gemm_fp8(ragged, transa, transb, m, n, k, groups, sm_count, ctypes.byref(bn), ctypes.byref(cg),
+                              ctypes.byref(parts))
+    return s, bn.value, cg.value, parts.value
+
+
+def moe_rows(tokens: int, experts: int, top_k: int, align: int = 1) -> int:
+    """gs_moe_rows: rows a plan of moe_route can need (the length of row_slot)."""
+    out = ctypes.c_int(0)
+    s = _lib.gs_moe_rows(tokens, experts, top_k, align, ctypes.byref(out))
+    if s != STATUS_SUCCESS:
+        raise GemmError(s, "gs_moe_rows")
+    return out.value
+
+
+def moe_route_workspace(tokens: int, experts: int, top_k: int) -> int:
+    """gs_moe_route_workspace: bytes of workspace moe_route needs for a plan (0 for few slots)."""
+    out = ctypes.c_size_t(0)
+    s = _lib.gs_moe_route_workspace(tokens, experts, top_k, ctypes.byref(out))
+    if s != STATUS_SUCCESS:
+        raise GemmError(s, "gs_moe_route_workspace")
+    return out.value
 
 
 def _ptr(x) -> int | None:
@@ -373,6 +439,82 @@ class Handle:
                                     algo)
         if check:
             self._check(s, "gs_gemm_batched_ex")
+        return s
+
+    # ---- block-scaled FP8 products and routed experts (device pointers / torch CUDA tensors) ----
+    def fp8_quantize(self, mode, axis, rows, cols, src, src_type, ld_src, dst, dst_type, ld_dst, scale, ld_scale,
+                     index=None, index_div=1, src_cols=0, check=True) -> int:
+        """Column-major rows x cols `src` to FP8 `dst` with power-of-two scales; see gs_fp8_quantize."""
+        s = _lib.gs_fp8_quantize(self._h, mode, axis, rows, cols, _ptr(src), src_type, ld_src, _ptr(index), index_div,
+                                 src_cols, _ptr(dst), dst_type, ld_dst, _ptr(scale), ld_scale)
+        if check:
+            self._check(s, "gs_fp8_quantize")
+        return s
+
+    def gemm_fp8(self, transa, transb, m, n, k, alpha, A, atype, lda, a_scale, a_mode, ldsa, B, btype, ldb, b_scale,
+                 b_mode, ldsb, beta, C, ctype, ldc, check=True) -> int:
+        a, b = ctypes.c_float(alpha), ctypes.c_float(beta)
+        s = _lib.gs_gemm_fp8(self._h, transa, transb, m, n, k, ctypes.byref(a), _ptr(A), atype, lda, _ptr(a_scale),
+                             a_mode, ldsa, _ptr(B), btype, ldb, _ptr(b_scale), b_mode, ldsb, ctypes.byref(b), _ptr(C),
+                             ctype, ldc)
+        if check:
+            self._check(s, "gs_gemm_fp8")
+        return s
+
+    def gemm_fp8_grouped(self, ragged, transa, transb, m, n, k, groups, offsets, alpha, A, atype, lda, stride_a, a_scale,
+                         a_mode, ldsa, stride_sa, B, btype, ldb, b_scale, b_mode, ldsb, beta, C, ctype, ldc, stride_c,
+                         check=True) -> int:
+        """offsets: groups + 1 int32 device values along the ragged axis (GROUP_N: columns of B and C; GROUP_K: K)."""
+        a, b = ctypes.c_float(alpha), ctypes.c_float(beta)
+        s = _lib.gs_gemm_fp8_grouped(self._h, ragged, transa, transb, m, n, k, groups, _ptr(offsets), ctypes.byref(a),
+                                     _ptr(A), atype, lda, stride_a, _ptr(a_scale), a_mode, ldsa, stride_sa, _ptr(B),
+                                     btype, ldb, _ptr(b_scale), b_mode, ldsb, ctypes.byref(b), _ptr(C), ctype, ldc,
+                                     stride_c)
+        if check:
+            self._check(s, "gs_gemm_fp8_grouped")
+        return s
+
+    def moe_route(self, tokens, experts, top_k, logits, logits_type, ld_logits, ids, weights, bias=None,
+                  score=ROUTE_SOFTMAX, groups=1, top_groups=1, renormalize=False, scale=1.0, token_count=None, align=1,
+                  offsets=None, slot_row=None, row_slot=None, rows=0, workspace=None, workspace_bytes=0,
+                  check=True) -> int:
+        """Expert choice and weights, and with `offsets` the row plan of the grouped products; see gs_moe_route."""
+        d = RouteDesc(tokens, experts, top_k, _ptr(logits), logits_type, ld_logits, _ptr(bias), score, groups,
+                      top_groups, int(renormalize), scale, _ptr(token_count), align, _ptr(ids), _ptr(weights),
+                      _ptr(offsets), _ptr(slot_row), _ptr(row_slot), rows, _ptr(workspace), workspace_bytes)
+        s = _lib.gs_moe_route(self._h, ctypes.byref(d))
+        if check:
+            self._check(s, "gs_moe_route")
+        return s
+
+    def moe_route_backward(self, tokens, experts, top_k, logits, logits_type, ld_logits, ids, dweights, dlogits,
+                           dlogits_type, ld_dlogits, score=ROUTE_SOFTMAX, renormalize=False, scale=1.0,
+                           check=True) -> int:
+        d = RouteDesc(tokens=tokens, experts=experts, top_k=top_k, logits=_ptr(logits), logits_type=logits_type,
+                      ld_logits=ld_logits, score=score, renormalize=int(renormalize), scale=scale, ids=_ptr(ids))
+        s = _lib.gs_moe_route_backward(self._h, ctypes.byref(d), _ptr(dweights), _ptr(dlogits), dlogits_type, ld_dlogits)
+        if check:
+            self._check(s, "gs_moe_route_backward")
+        return s
+
+    def moe_combine(self, tokens, top_k, hidden, y, ytype, ldy, rows, slot_row, weights, out, out_type, ld_out,
+                    check=True) -> int:
+        s = _lib.gs_moe_combine(self._h, tokens, top_k, hidden, _ptr(y), ytype, ldy, rows, _ptr(slot_row),
+                                _ptr(weights), _ptr(out), out_type, ld_out)
+        if check:
+            self._check(s, "gs_moe_combine")
+        return s
+
+    def moe_combine_backward(self, tokens, top_k, hidden, y, ytype, ldy, rows, slot_row, row_slot, weights, dout,
+                             dout_type, ld_dout, dy, ld_dy, dweights, check=True) -> int:
+        """dout and dy have y's type (dout_type must be ytype)."""
+        if dout_type != ytype:
+            raise ValueError("dout must have y's type")
+        s = _lib.gs_moe_combine_backward(self._h, tokens, top_k, hidden, _ptr(y), ytype, ldy, rows, _ptr(slot_row),
+                                         _ptr(row_slot), _ptr(weights), _ptr(dout), ld_dout, _ptr(dy), ld_dy,
+                                         _ptr(dweights))
+        if check:
+            self._check(s, "gs_moe_combine_backward")
         return s
 
     # ---- host-buffer mirror of gemm.gemmEx ----
