@@ -1,25 +1,39 @@
 // gemm_fp8_sm100.cu -- FP8 matrix products with one f32 scale per 128 elements
 // along K (or per 128 x 128 block), dense and over ragged groups, for sm_100a.
 //
-//   C[i, j] = alpha * sum_b sA(i, b) * sB(j, b) * P_b[i, j] + beta * C[i, j],
-//   P_b[i, j] = sum over the 128 K elements of block b of op(A)[i, p] * op(B)[p, j]
+//   C[i, j] = alpha * sum_b sA(i, b) * sB(j, b) * S_b[i, j] + beta * C[i, j],
+//   S_b[i, j] = sum over the 128 K elements of block b of op(A)[i, p] * op(B)[p, j]
 //
 // The scales are arbitrary f32 numbers, so they cannot be folded into the
-// tensor core's accumulation over K: each block's P_b is computed by four
+// tensor core's accumulation over K: each block's S_b is computed by four
 // tcgen05.mma (kind::f8f6f4, K = 32) into a TMEM slot of its own, and the
-// epilogue warps ("promoters") read the slot and add scale * P_b to f32 sums
+// epilogue warps ("promoters") read the slot and add scale * S_b to f32 sums
 // in registers with packed FMAs while the tensor core fills the next slot.
 // Products of two FP8 values are exact in f32 and a block sums 128 of them.
 //
+// A tile is P rows (TMEM lanes, one per promoter thread) by Q columns. Two
+// orientations:
+//  - wide tiles (BN = 256): P = op(B)'s columns (tokens), Q = op(A)'s rows
+//    (features). With tokens scaled per vector and weights per block a thread's
+//    scale of a K block is one number, and a thread's row of C is contiguous, so
+//    C leaves through 128-byte swizzled staging and TMA stores. CTA pairs
+//    (cta_group::2) compute 256 x 256.
+//  - narrow tiles (BN = 32, 64, 128; few tokens, bound by reading A): P = op(A)'s
+//    rows, Q = op(B)'s columns, so no row of the tensor core is spent on
+//    tokens that are not there; 32 lanes store 32 consecutive rows of C.
+// A scale per Q column is the same for all lanes: it is read from shared memory
+// as a broadcast, and costs one more packed multiply.
+//
 // One CTA (or CTA pair) per SM runs tiles persistently:
-//  - warp 0: TMA producer, 128 x 128 bytes of A and BN / CG x 128 of B a stage;
+//  - warp 0: TMA producer, 128 x 128 bytes of P and BN / CG x 128 of Q a stage;
 //    transposes live in the tensor maps and the UMMA major bits;
 //  - warp 1: TMEM allocation, and tcgen05.mma from one thread (even CTA);
-//  - warp 2: copies each K block's scales into a ring in shared memory;
-//  - warps 4..: promoters, one accumulator row per thread, BN / (warps / 4)
-//    columns each. With 128 columns a thread they need more registers than an
-//    even split gives: of the 3 x 168 a lane triple is launched with, the first
-//    warpgroup hands 96 to the two promoter warpgroups (72 / 216 / 216).
+//  - warp 2: copies each K block's scales into a ring in shared memory with
+//    cp.async, which completes on the ring's mbarriers;
+//  - warps 4..: promoters, BN / (warps / 4) columns each. With 128 columns a
+//    thread they need more registers than an even split gives: of the 3 x 168 a
+//    lane triple is launched with, the first warpgroup hands 96 to the two
+//    promoter warpgroups (72 / 216 / 216).
 // Ragged groups: offsets are read from device memory; tile counts are scanned
 // once per CTA into shared memory and each tile finds its group by bisection.
 //
@@ -29,6 +43,7 @@
 #include <type_traits>
 
 #include "gs_epilogue.cuh"
+#include "gs_float.cuh"
 #include "gs_fp8.h"
 #include "gs_internal.h"
 #include "gs_ptx.cuh"
@@ -42,66 +57,75 @@ constexpr int SC_STAGES = 8;
 
 template <int CG, int BN>
 struct Cfg {
+    static constexpr bool WIDE = BN == 256;  // P = B's columns, Q = A's rows
     static constexpr int EPI_WARPS = BN >= 128 ? 8 : 4;
     static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
-    static constexpr int B_ROWS = BN / CG;
-    static constexpr int A_STAGE = BM * BK;
-    static constexpr int B_STAGE = B_ROWS * BK;
-    static constexpr int STAGE = A_STAGE + B_STAGE;
-    static constexpr int STAGES = STAGE >= 48 * 1024 ? 4 : (STAGE >= 32 * 1024 ? 6 : 8);
+    static constexpr int Q_ROWS = BN / CG;
+    static constexpr int P_STAGE = BM * BK;
+    static constexpr int Q_STAGE = Q_ROWS * BK;
+    static constexpr int STAGE = P_STAGE + Q_STAGE;
+    static constexpr int STAGES = WIDE ? (CG == 2 ? 5 : 3) : (STAGE >= 32 * 1024 ? 6 : 8);
+    static constexpr int STG_BLOCK = 32 * 128;  // a promoter warp's staging: 32 rows of 128 bytes
+    static constexpr int STG_BYTES = WIDE ? EPI_WARPS * STG_BLOCK : 0;
     static constexpr int SLOTS = BN == 256 ? 2 : 4;
     static constexpr int TMEM_COLS = BN * SLOTS;
     static constexpr int SC_FLOATS = BN + BM;
-    static constexpr int TILE_M = BM * CG;
+    static constexpr int TILE_P = BM * CG;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 2 * SC_STAGES + 1;
-    static constexpr int SMEM = STAGES * STAGE + SC_STAGES * SC_FLOATS * 4 + BARS * 8 + 16 + 1024 /*alignment*/;
+    static constexpr int SMEM = STAGES * STAGE + STG_BYTES + SC_STAGES * SC_FLOATS * 4 + BARS * 8 + 16 + 1024 /*alignment*/;
+};
+
+// One operand as the kernel sees it: `extent` rows (P) or columns (Q) besides K.
+struct Side {
+    int extent;
+    int mn;                    // stored with the non-K axis contiguous
+    int grouped;               // the tensor map's third coordinate is the group
+    const float *scale;
+    long long s_i, s_k, s_g;   // element strides: index (or its block of 128), K block, group
 };
 
 struct Args {
-    int m, n, k;
-    int m_blocks, n_blocks, k_blocks;  // n_blocks: of the dense / ragged-K product
+    Side p, q;
+    int k;
+    int p_blocks, q_blocks, k_blocks;  // tiles along each axis (of the ragged one: unused)
     int groups;                        // 0 = dense
-    int ragged;                        // GS_GROUP_N / GS_GROUP_K when groups > 0
+    int ragged;                        // GS_GROUP_N / GS_GROUP_K, -1 = dense
     const int32_t *offsets;
-    int group_m;
     int split;                         // cluster CTAs sharing a tile's K blocks (1 = none)
-    long long total_tiles;             // dense and ragged-K
-    int a_mn, b_mn;
-    int a_bcast;                       // every group multiplies by the same A
+    long long total_tiles;             // dense and ragged K
     uint32_t idesc;
-    const float *sa;
-    long long sa_i, sa_k, sa_g;        // element strides: row or row block, K block, group
-    const float *sb;
-    long long sb_i, sb_k;
     void *C;
     long long ldc, stride_c;
     int out_kind;
+    int tma_store;                     // C can be written through tmC
+    int vec_c;                         // C's rows can be read and written 16 bytes at a time
     Epilogue ep;
     uint32_t *err;
     long long spin_limit;
 };
 
-// A tile: rows m0.. of group g, columns n0..n_end, K blocks kb0..kb0+nkb.
+// A tile of group g: rows p0.. (p_end: behind the last), columns q0.., K blocks kb0..kb0+nkb.
 struct Item {
-    int g, m0, n0, n_end, kb0, nkb;
+    int g, p0, p_end, q0, q_end, kb0, nkb;
     bool bad;  // ragged-K group whose offsets are not multiples of 128
 };
+
+constexpr int RASTER = 8;  // rows of tiles visited together, so that concurrent tiles share operands in L2
 
 template <int CG, int BN>
 __device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, const int *off, long long t, uint32_t rank,
                                         Item &it) {
-    int mb, nb, n_blocks = a.n_blocks;
+    using C_ = Cfg<CG, BN>;
+    int p_blocks = a.p_blocks, q_blocks = a.q_blocks, p_base = 0, q_base = 0;
     long long r = t;
     it.g = 0;
     it.bad = false;
     it.kb0 = 0;
     it.nkb = a.k_blocks;
-    int n_base = 0;
-    it.n_end = a.n;
-    if (a.groups == 0) {
-        if (t >= a.total_tiles) return false;
-    } else if (a.ragged == GS_GROUP_N) {
+    it.p_end = a.p.extent;
+    it.q_end = a.q.extent;
+    if (a.ragged == GS_GROUP_N) {
         if (t >= tile_start[a.groups]) return false;
         int lo = 0, hi = a.groups;  // the last group whose first tile is <= t
         while (hi - lo > 1) {
@@ -111,29 +135,36 @@ __device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, co
         }
         it.g = lo;
         r = t - tile_start[lo];
-        n_base = off[lo];
-        it.n_end = off[lo + 1];
-        n_blocks = (it.n_end - n_base + BN - 1) / BN;
+        if (C_::WIDE) {
+            p_base = off[lo];
+            it.p_end = off[lo + 1];
+            p_blocks = (it.p_end - p_base + C_::TILE_P - 1) / C_::TILE_P;
+        } else {
+            q_base = off[lo];
+            it.q_end = off[lo + 1];
+            q_blocks = (it.q_end - q_base + BN - 1) / BN;
+        }
     } else {
         if (t >= a.total_tiles) return false;
-        const long long per = static_cast<long long>(a.m_blocks) * a.n_blocks;
-        it.g = static_cast<int>(t / per);
-        r = t - it.g * per;
-        const int k_lo = off[it.g], k_hi = off[it.g + 1];
-        it.kb0 = k_lo / BK;
-        it.nkb = (k_hi - k_lo + BK - 1) / BK;
-        it.bad = k_hi > k_lo && (k_lo % BK != 0 || (k_hi % BK != 0 && k_hi != a.k));
-        if (it.bad) it.nkb = 0;
+        if (a.ragged == GS_GROUP_K) {
+            const long long per = static_cast<long long>(p_blocks) * q_blocks;
+            it.g = static_cast<int>(t / per);
+            r = t - it.g * per;
+            const int k_lo = off[it.g], k_hi = off[it.g + 1];
+            it.kb0 = k_lo / BK;
+            it.nkb = (k_hi - k_lo + BK - 1) / BK;
+            it.bad = k_hi > k_lo && (k_lo % BK != 0 || (k_hi % BK != 0 && k_hi != a.k));
+            if (it.bad) it.nkb = 0;
+        }
     }
-    const long long span = static_cast<long long>(a.group_m) * n_blocks;
+    const int height = p_blocks < RASTER ? p_blocks : RASTER;
+    const long long span = static_cast<long long>(height) * q_blocks;
     const int gi = static_cast<int>(r / span);
     const int within = static_cast<int>(r - gi * span);
-    const int first = gi * a.group_m;
-    const int gm = min(a.group_m, a.m_blocks - first);
-    mb = first + within % gm;
-    nb = within / gm;
-    it.m0 = mb * Cfg<CG, BN>::TILE_M + static_cast<int>(CG == 2 ? rank : 0) * BM;
-    it.n0 = n_base + nb * BN;
+    const int first = gi * height;
+    const int rows = min(height, p_blocks - first);
+    it.p0 = p_base + (first + within % rows) * C_::TILE_P + static_cast<int>(CG == 2 ? rank : 0) * BM;
+    it.q0 = q_base + within / rows * BN;
     if (CG == 1 && a.split > 1) {  // this CTA's share of the K blocks
         const int lo = static_cast<int>(static_cast<long long>(it.nkb) * rank / a.split);
         const int hi = static_cast<int>(static_cast<long long>(it.nkb) * (rank + 1) / a.split);
@@ -194,38 +225,81 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
+// 4-byte asynchronous copy global -> shared; zeros where `in` is false.
+__device__ __forceinline__ void cp_async_f32(uint32_t dst, const float *src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// Arrives on the barrier when this thread's earlier cp.async have completed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 // One element of C, rounded once from f32 (to nearest even).
+template <typename T>
+__device__ __forceinline__ void store_one(const Args &a, T *c, float v) {
+    if (!a.ep.beta_zero) v = __fmaf_rn(a.ep.beta_f, to_f32(*c), v);
+    *c = from_f32<T>(v);
+}
+__device__ __forceinline__ float scaled(const Args &a, float acc) { return a.ep.identity ? acc : __fmul_rn(a.ep.alpha_f, acc); }
 __device__ __forceinline__ void store_c(const Args &a, void *C, size_t i, float acc) {
-    float v = a.ep.identity ? acc : __fmul_rn(a.ep.alpha_f, acc);
-    if (a.out_kind == OUT_F32) {
-        float *c = static_cast<float *>(C) + i;
-        if (!a.ep.beta_zero) v = __fmaf_rn(a.ep.beta_f, *c, v);
-        *c = v;
-    } else if (a.out_kind == OUT_F16) {
-        __half *c = static_cast<__half *>(C) + i;
-        if (!a.ep.beta_zero) v = __fmaf_rn(a.ep.beta_f, __half2float(*c), v);
-        *c = __float2half_rn(v);
-    } else {
-        __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(C) + i;
-        if (!a.ep.beta_zero) v = __fmaf_rn(a.ep.beta_f, __bfloat162float(*c), v);
-        *c = __float2bfloat16_rn(v);
+    const float v = scaled(a, acc);
+    if (a.out_kind == OUT_F32) store_one(a, static_cast<float *>(C) + i, v);
+    else if (a.out_kind == OUT_F16) store_one(a, static_cast<__half *>(C) + i, v);
+    else store_one(a, static_cast<__nv_bfloat16 *>(C) + i, v);
+}
+// C of group g (ragged K).
+__device__ __forceinline__ void *group_c(const Args &a, int g) {
+    if (a.ragged != GS_GROUP_K) return a.C;
+    return static_cast<uint8_t *>(a.C) + static_cast<size_t>(g) * a.stride_c * (a.out_kind == OUT_F32 ? 4 : 2);
+}
+
+// 128 consecutive elements of one row of C from a thread's sums (alpha applied), `n` of them inside.
+template <typename T>
+__device__ __forceinline__ void store_row(const Args &a, T *c, int n, const uint64_t (&acc)[64]) {
+#pragma unroll
+    for (int j = 0; j < 128; j += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2(acc[j / 2 + i], v[2 * i], v[2 * i + 1]);
+        if (a.vec_c && j + 8 <= n) {
+            Pack<T, 8> out;
+            if (!a.ep.beta_zero) {
+                const Pack<T, 8> old = load_pack<T, 8>(c + j);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __fmaf_rn(a.ep.beta_f, to_f32(old.v[i]), v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out.v[i] = from_f32<T>(v[i]);
+            store_pack<T, 8>(c + j, out);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i < n) store_one(a, c + j + i, v[i]);
+        }
     }
 }
 
-// MODE bit 0: A has a scale per row (else per 128 rows); bit 1: B has a scale
+// MODE bit 0: P has a scale per row (else per 128 rows); bit 1: Q has a scale
 // per column (else per 128 columns).
 template <int CG, int BN, int MODE>
 __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
-    k_gemm_fp8(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
+    k_gemm_fp8(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+               const __grid_constant__ CUtensorMap tmC, const Args args) {
     using C_ = Cfg<CG, BN>;
-    constexpr bool A_VEC = (MODE & 1) != 0, B_VEC = (MODE & 2) != 0;
+    constexpr bool P_VEC = (MODE & 1) != 0, Q_VEC = (MODE & 2) != 0;
     constexpr int STAGES = C_::STAGES, SLOTS = C_::SLOTS, EPI_COLS = C_::EPI_COLS;
 
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *smA = smem;
-    uint8_t *smB = smem + STAGES * C_::A_STAGE;
-    float *scales = reinterpret_cast<float *>(smB + STAGES * C_::B_STAGE);
+    uint8_t *smP = smem;
+    uint8_t *smQ = smem + STAGES * C_::P_STAGE;
+    uint8_t *stg = smQ + STAGES * C_::Q_STAGE;
+    float *scales = reinterpret_cast<float *>(stg + C_::STG_BYTES);
     uint64_t *full = reinterpret_cast<uint64_t *>(scales + SC_STAGES * C_::SC_FLOATS);
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
@@ -260,8 +334,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0 && args.k_blocks > 0) {
-        prefetch_tensormap(&tmA);
-        prefetch_tensormap(&tmB);
+        prefetch_tensormap(&tmP);
+        prefetch_tensormap(&tmQ);
     }
     if (warp == 1) {
         if constexpr (CG == 2) {
@@ -276,7 +350,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     if (warp == 2 && args.groups > 0) {
         // Clamped, never decreasing offsets (whatever the caller's memory holds, every access stays inside the
         // operands) and, for ragged N, the running count of tiles.
-        const int limit = args.ragged == GS_GROUP_N ? args.n : args.k;
+        const int limit = args.ragged == GS_GROUP_K ? args.k : C_::WIDE ? args.p.extent : args.q.extent;
         const int per = (args.groups + 32) / 32;  // of groups + 1 offsets
         const int lo = min(lane * per, args.groups + 1), hi = min(lo + per, args.groups + 1);
         int top = 0;
@@ -294,10 +368,12 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         for (int i = lo; i < hi; ++i) off[i] = max(off[i], before);
         __syncwarp();
         if (args.ragged == GS_GROUP_N) {
+            constexpr int TILE = C_::WIDE ? C_::TILE_P : BN;
+            const int across = C_::WIDE ? args.q_blocks : args.p_blocks;
             int sum = 0;
             for (int i = lo; i < hi; ++i) {
                 tile_start[i] = sum;
-                if (i < args.groups) sum += (off[i + 1] - off[i] + BN - 1) / BN * args.m_blocks;
+                if (i < args.groups) sum += (off[i + 1] - off[i] + TILE - 1) / TILE * across;
             }
             int incl = sum;
             for (int d = 1; d < 32; d <<= 1) {
@@ -321,36 +397,37 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     if (warp < 4) {
     if constexpr (EPI_COLS == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
+        // ---------------- TMA producer ----------------
         if (lane == 0) {
             const uint64_t pol = l2_policy_evict_normal();
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
-                const int nc = it.n0 + static_cast<int>(CG == 2 ? rank : 0) * C_::B_ROWS;
-                const int ga = args.a_bcast ? 0 : it.g;
+                const int qc = it.q0 + static_cast<int>(CG == 2 ? rank : 0) * C_::Q_ROWS;
+                const int gp = args.p.grouped ? it.g : 0, gq = args.q.grouped ? it.g : 0;
                 for (int kb = 0; kb < it.nkb; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, 1, args.spin_limit)) { ok = false; break; }
-                    uint8_t *dA = smA + stage * C_::A_STAGE;
-                    uint8_t *dB = smB + stage * C_::B_STAGE;
+                    uint8_t *dP = smP + stage * C_::P_STAGE;
+                    uint8_t *dQ = smQ + stage * C_::Q_STAGE;
                     const int k0 = (it.kb0 + kb) * BK;
                     if constexpr (CG == 2) {
                         const uint32_t fbar = mapa_shared(smem_u32(&full[stage]), 0);
                         if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C_::STAGE);
-                        if (args.a_mn) tma_load_3d_2sm(dA, &tmA, fbar, it.m0, k0, ga, pol);
-                        else tma_load_3d_2sm(dA, &tmA, fbar, k0, it.m0, ga, pol);
-                        if (args.b_mn) tma_load_3d_2sm(dB, &tmB, fbar, nc, k0, 0, pol);
-                        else tma_load_3d_2sm(dB, &tmB, fbar, k0, nc, 0, pol);
+                        if (args.p.mn) tma_load_3d_2sm(dP, &tmP, fbar, it.p0, k0, gp, pol);
+                        else tma_load_3d_2sm(dP, &tmP, fbar, k0, it.p0, gp, pol);
+                        if (args.q.mn) tma_load_3d_2sm(dQ, &tmQ, fbar, qc, k0, gq, pol);
+                        else tma_load_3d_2sm(dQ, &tmQ, fbar, k0, qc, gq, pol);
                     } else {
                         mbar_arrive_expect_tx(&full[stage], C_::STAGE);
-                        if (args.a_mn) tma_load_3d_hint(dA, &tmA, &full[stage], it.m0, k0, ga, pol);
-                        else tma_load_3d_hint(dA, &tmA, &full[stage], k0, it.m0, ga, pol);
-                        if (args.b_mn) {  // only with BN >= 128: panels of 128 columns
+                        if (args.p.mn) tma_load_3d_hint(dP, &tmP, &full[stage], it.p0, k0, gp, pol);
+                        else tma_load_3d_hint(dP, &tmP, &full[stage], k0, it.p0, gp, pol);
+                        if (args.q.mn) {  // only with BN >= 128: panels of 128 columns
 #pragma unroll
                             for (int c = 0; c < (BN + 127) / 128; ++c)
-                                tma_load_3d_hint(dB + c * 128 * BK, &tmB, &full[stage], nc + c * 128, k0, 0, pol);
+                                tma_load_3d_hint(dQ + c * 128 * BK, &tmQ, &full[stage], qc + c * 128, k0, gq, pol);
                         } else {
-                            tma_load_3d_hint(dB, &tmB, &full[stage], k0, nc, 0, pol);
+                            tma_load_3d_hint(dQ, &tmQ, &full[stage], k0, qc, gq, pol);
                         }
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -358,6 +435,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
             }
         }
     } else if (warp == 1) {
+        // ---------------- MMA issuer (even CTA) ----------------
         if (lane == 0 && leader) {
             int stage = 0, slot = 0;
             uint32_t phase = 0, sphase = 0;
@@ -370,15 +448,15 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a_base = smem_u32(smA + stage * C_::A_STAGE);
-                    const uint32_t b_base = smem_u32(smB + stage * C_::B_STAGE);
+                    const uint32_t p_base = smem_u32(smP + stage * C_::P_STAGE);
+                    const uint32_t q_base = smem_u32(smQ + stage * C_::Q_STAGE);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t adesc = args.a_mn ? umma_smem_desc_sw128(a_base + kk * 32 * 128, 128 * BK, 1024)
-                                                         : umma_smem_desc_sw128(a_base + kk * 32, 16, 1024);
-                        const uint64_t bdesc = args.b_mn ? umma_smem_desc_sw128(b_base + kk * 32 * 128, 128 * BK, 1024)
-                                                         : umma_smem_desc_sw128(b_base + kk * 32, 16, 1024);
-                        umma_f8<CG>(tmem_base + slot * BN, adesc, bdesc, args.idesc, kk != 0 ? 1u : 0u);
+                        const uint64_t pdesc = args.p.mn ? umma_smem_desc_sw128(p_base + kk * 32 * 128, 128 * BK, 1024)
+                                                         : umma_smem_desc_sw128(p_base + kk * 32, 16, 1024);
+                        const uint64_t qdesc = args.q.mn ? umma_smem_desc_sw128(q_base + kk * 32 * 128, 128 * BK, 1024)
+                                                         : umma_smem_desc_sw128(q_base + kk * 32, 16, 1024);
+                        umma_f8<CG>(tmem_base + slot * BN, pdesc, qdesc, args.idesc, kk != 0 ? 1u : 0u);
                     }
                     if constexpr (CG == 2) {
                         umma_commit_2sm(&empty[stage], 0x3);
@@ -398,56 +476,50 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
             }
         }
     } else if (warp == 2) {
-        // Scales. A few K blocks are fetched at a time so that their loads overlap.
-        constexpr int NB = B_VEC ? BN / 32 : 1, NA = A_VEC ? BM / 32 : 1, U = EPI_COLS == 128 ? 2 : 4;
+        // ---------------- scales: [BN] of Q (per column, or one per 128), then [128] (or one) of P ----------------
         int ss = 0;
         uint32_t sp = 0;
         bool ok = true;
         for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
-            const float *pa = args.sa + it.g * args.sa_g;
-            for (int kb = 0; ok && kb < it.nkb; kb += U) {
-                float va[U][NA], vb[U][NB];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const long long ka = it.kb0 + min(kb + u, it.nkb - 1);
-#pragma unroll
-                    for (int i = 0; i < NA; ++i) {
-                        const int r = A_VEC ? it.m0 + i * 32 + lane : it.m0 / 128;
-                        const bool in = A_VEC ? r < args.m : it.m0 < args.m;
-                        va[u][i] = in ? pa[r * args.sa_i + ka * args.sa_k] : 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const int c = B_VEC ? it.n0 + i * 32 + lane : it.n0 / 128 + lane;
-                        const bool in = B_VEC ? c < it.n_end : (lane < (BN + 127) / 128 && it.n0 + lane * 128 < args.n);
-                        vb[u][i] = in ? args.sb[c * args.sb_i + ka * args.sb_k] : 0.0f;
-                    }
+            const float *pp = args.p.scale + it.g * args.p.s_g, *pq = args.q.scale + it.g * args.q.s_g;
+            for (int kb = 0; kb < it.nkb; ++kb) {
+                // one answer for the warp: its lanes arrive together
+                if (!__all_sync(0xffffffffu, mbar_wait(&sempty[ss], sp ^ 1u, args.err, 6, args.spin_limit))) {
+                    ok = false;
+                    break;
                 }
+                const uint32_t dst = smem_u32(scales + ss * C_::SC_FLOATS);
+                const long long k = it.kb0 + kb;
+                if constexpr (Q_VEC) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (!ok || kb + u >= it.nkb) break;
-                    // one answer for the warp: its lanes arrive together
-                    if (!__all_sync(0xffffffffu, mbar_wait(&sempty[ss], sp ^ 1u, args.err, 6, args.spin_limit))) {
-                        ok = false;
-                        break;
+                    for (int i = 0; i < BN / 32; ++i) {
+                        const int c = it.q0 + i * 32 + lane;
+                        const bool in = c < it.q_end;
+                        cp_async_f32(dst + (i * 32 + lane) * 4, in ? pq + c * args.q.s_i + k * args.q.s_k : pq, in);
                     }
-                    float *dst = scales + ss * C_::SC_FLOATS;
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const float v = A_VEC ? vb[u][i] : __fmul_rn(va[u][0], vb[u][i]);
-                        if (B_VEC || lane < (BN + 127) / 128) dst[i * 32 + lane] = v;
-                    }
-                    if constexpr (A_VEC) {
-#pragma unroll
-                        for (int i = 0; i < NA; ++i) dst[BN + i * 32 + lane] = va[u][i];
-                    }
-                    mbar_arrive(&sfull[ss]);
-                    if (++ss == SC_STAGES) { ss = 0; sp ^= 1u; }
+                } else if (lane < (BN + 127) / 128) {
+                    const bool in = it.q0 + lane * 128 < it.q_end;
+                    cp_async_f32(dst + lane * 4, in ? pq + (it.q0 / 128 + lane) * args.q.s_i + k * args.q.s_k : pq, in);
                 }
+                if constexpr (P_VEC) {
+#pragma unroll
+                    for (int i = 0; i < BM / 32; ++i) {
+                        const int r = it.p0 + i * 32 + lane;
+                        const bool in = r < it.p_end;
+                        cp_async_f32(dst + (BN + i * 32 + lane) * 4, in ? pp + r * args.p.s_i + k * args.p.s_k : pp, in);
+                    }
+                } else if (lane == 0) {
+                    const bool in = it.p0 < it.p_end;
+                    cp_async_f32(dst + BN * 4, in ? pp + it.p0 / 128 * args.p.s_i + k * args.p.s_k : pp, in);
+                }
+                cp_async_arrive(&sfull[ss]);
+                if (++ss == SC_STAGES) { ss = 0; sp ^= 1u; }
             }
         }
+        cp_async_wait_all();
     }
     } else {
+        // ---------------- promoters ----------------
         if constexpr (EPI_COLS == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quad = warp & 3;
         const int ew = warp - 4;
@@ -455,6 +527,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         const int row = quad * 32 + lane;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
         const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(&tempty[0]), 0) : 0u;
+        const uint64_t pol_c = l2_policy_evict_first();
         int slot = 0, ss = 0;
         uint32_t phase = 0, sp = 0;
         bool ok = true;
@@ -475,23 +548,22 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                     break;
                 }
                 tc_fence_after();
+                // The next 32 columns are on their way while these are added.
+                const uint32_t t_slot = t_lane + slot * BN + c_lo;
+                uint32_t r[2][32];
+                tmem_ld_32x32b_x32(t_slot, r[0]);
                 const float *sc = scales + ss * C_::SC_FLOATS;
                 const uint32_t sc_addr = smem_u32(sc + c_lo);
-                uint64_t sa2 = 0;
-                if constexpr (A_VEC && B_VEC) {
-                    const float sa = sc[BN + row];
-                    sa2 = pack2(sa, sa);
-                } else if constexpr (!B_VEC) {
-                    float s = sc[c_lo / 128];
-                    if constexpr (A_VEC) s = __fmul_rn(sc[BN + row], s);
-                    sa2 = pack2(s, s);
-                }
+                float s = sc[BN + (P_VEC ? row : 0)];
+                if constexpr (!Q_VEC) s = __fmul_rn(s, sc[c_lo / 128]);
+                const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int c = 0; c < EPI_COLS; c += 32) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(t_lane + slot * BN + c_lo + c, r);
+                    const int cur = (c / 32) & 1;
                     tmem_wait_ld();
-                    if (c + 32 == EPI_COLS) {  // the slot is read: the tensor core may fill it again
+                    if (c + 32 < EPI_COLS) {
+                        tmem_ld_32x32b_x32(t_slot + c + 32, r[cur ^ 1]);
+                    } else {  // the slot is read: the tensor core may fill it again
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -501,19 +573,16 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        uint64_t p0 = pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-                        uint64_t p1 = pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-                        if constexpr (B_VEC) {
+                        const uint64_t p0 = pack2(__uint_as_float(r[cur][j]), __uint_as_float(r[cur][j + 1]));
+                        const uint64_t p1 = pack2(__uint_as_float(r[cur][j + 2]), __uint_as_float(r[cur][j + 3]));
+                        uint64_t &a0 = acc[(c + j) / 2], &a1 = acc[(c + j) / 2 + 1];
+                        if constexpr (Q_VEC) {
                             const float4 s4 = ld_shared_f32x4(sc_addr + (c + j) * 4);
-                            if constexpr (A_VEC) {
-                                p0 = mul2(p0, sa2);
-                                p1 = mul2(p1, sa2);
-                            }
-                            acc[(c + j) / 2] = fma2(p0, pack2(s4.x, s4.y), acc[(c + j) / 2]);
-                            acc[(c + j) / 2 + 1] = fma2(p1, pack2(s4.z, s4.w), acc[(c + j) / 2 + 1]);
+                            a0 = fma2(mul2(p0, s2), pack2(s4.x, s4.y), a0);
+                            a1 = fma2(mul2(p1, s2), pack2(s4.z, s4.w), a1);
                         } else {
-                            acc[(c + j) / 2] = fma2(p0, sa2, acc[(c + j) / 2]);
-                            acc[(c + j) / 2 + 1] = fma2(p1, sa2, acc[(c + j) / 2 + 1]);
+                            a0 = fma2(p0, s2, a0);
+                            a1 = fma2(p1, s2, a1);
                         }
                     }
                 }
@@ -523,53 +592,123 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                 if (++ss == SC_STAGES) { ss = 0; sp ^= 1u; }
             }
             if (!ok) break;
-            if (CG == 1 && args.split > 1) {
-                // This slice's sums, column by column, over the operand stages: every load has landed and every
-                // MMA that read them has committed.
-                const uint32_t base = smem_u32(smem) + (c_lo * BM + row) * 4;
+            if constexpr (C_::WIDE) {
+                // Row p of C is contiguous. Whole warps go out through staging: 32 rows of 128 bytes, 16-byte chunks
+                // swizzled by the row so that neither side has bank conflicts; rows past a ragged group's end
+                // belong to the next group, which a TMA store would overwrite.
+                const int n = it.q_end - it.q0 - c_lo;
+                const int p = it.p0 + row, p_warp = it.p0 + quad * 32;
+                if (!args.ep.identity) {
+                    const uint64_t al = pack2(args.ep.alpha_f, args.ep.alpha_f);
 #pragma unroll
-                for (int j = 0; j < EPI_COLS / 2; ++j) {
-                    float x, y;
-                    unpack2(acc[j], x, y);
-                    st_shared_f32(base + (2 * j) * BM * 4, x);
-                    st_shared_f32(base + (2 * j + 1) * BM * 4, y);
+                    for (int j = 0; j < 64; ++j) acc[j] = mul2(acc[j], al);
                 }
-                break;  // one tile per cluster
-            }
-            const int m = it.m0 + row;
-            if (m < args.m) {
-                void *Cb = args.C;
-                if (args.ragged == GS_GROUP_K)
-                    Cb = static_cast<uint8_t *>(args.C) + static_cast<size_t>(it.g) * args.stride_c * (args.out_kind == OUT_F32 ? 4 : 2);
+                if (args.tma_store && (args.ragged != GS_GROUP_N || p_warp + 32 <= it.p_end)) {
+                    uint8_t *buf = stg + ew * C_::STG_BLOCK;
+                    const uint32_t dst = smem_u32(buf) + lane * 128;
+                    const int gc = args.ragged == GS_GROUP_K ? it.g : 0;
+                    // `words` packs the 16 bytes of chunk x of block b
+                    auto blocks = [&](auto cols_c, auto words) {
+                        constexpr int COLS = decltype(cols_c)::value;  // columns of 128 bytes
 #pragma unroll
-                for (int j = 0; j < EPI_COLS / 2; ++j) {
-                    float x, y;
-                    unpack2(acc[j], x, y);
-                    const int n = it.n0 + c_lo + 2 * j;
-                    const size_t i = static_cast<size_t>(m) + static_cast<size_t>(n) * args.ldc;
-                    if (n < it.n_end) store_c(args, Cb, i, x);
-                    if (n + 1 < it.n_end) store_c(args, Cb, i + args.ldc, y);
+                        for (int b = 0; b < 128 / COLS; ++b) {
+                            if (b * COLS >= n || p_warp >= it.p_end) break;
+                            if (lane == 0) bulk_wait_group_read<0>();
+                            __syncwarp();
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                uint32_t w[4];
+                                words(b * COLS + x * (COLS / 8), w);
+                                st_shared_v4(dst + ((x ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                            }
+                            fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) {
+                                tma_store_3d(&tmC, buf, it.q0 + c_lo + b * COLS, p_warp, gc, pol_c);
+                                bulk_commit_group();
+                            }
+                        }
+                    };
+                    if (args.out_kind == OUT_F32) {
+                        blocks(std::integral_constant<int, 32>{}, [&](int j, uint32_t (&w)[4]) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                float x, y;
+                                unpack2(acc[j / 2 + i], x, y);
+                                w[2 * i] = __float_as_uint(x);
+                                w[2 * i + 1] = __float_as_uint(y);
+                            }
+                        });
+                    } else {
+                        const bool half = args.out_kind == OUT_F16;
+                        blocks(std::integral_constant<int, 64>{}, [&](int j, uint32_t (&w)[4]) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float x, y;
+                                unpack2(acc[j / 2 + i], x, y);
+                                if (half) {
+                                    const __half2 h = __floats2half2_rn(x, y);
+                                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                                } else {
+                                    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                                }
+                            }
+                        });
+                    }
+                } else if (p < it.p_end && n > 0) {
+                    void *Cb = group_c(args, it.g);
+                    const size_t i = static_cast<size_t>(p) * args.ldc + it.q0 + c_lo;
+                    if (args.out_kind == OUT_F32) store_row(args, static_cast<float *>(Cb) + i, n, acc);
+                    else if (args.out_kind == OUT_F16) store_row(args, static_cast<__half *>(Cb) + i, n, acc);
+                    else store_row(args, static_cast<__nv_bfloat16 *>(Cb) + i, n, acc);
+                }
+            } else {
+                if (args.split > 1) {
+                    // This slice's sums, column by column, over the operand stages: every load has landed and every
+                    // MMA that read them has committed.
+                    const uint32_t base = smem_u32(smem) + (c_lo * BM + row) * 4;
+#pragma unroll
+                    for (int j = 0; j < EPI_COLS / 2; ++j) {
+                        float x, y;
+                        unpack2(acc[j], x, y);
+                        st_shared_f32(base + (2 * j) * BM * 4, x);
+                        st_shared_f32(base + (2 * j + 1) * BM * 4, y);
+                    }
+                    break;  // one tile per cluster
+                }
+                const int p = it.p0 + row;
+                if (p < it.p_end) {
+                    void *Cb = group_c(args, it.g);
+#pragma unroll
+                    for (int j = 0; j < EPI_COLS / 2; ++j) {
+                        float x, y;
+                        unpack2(acc[j], x, y);
+                        const int q = it.q0 + c_lo + 2 * j;
+                        const size_t i = static_cast<size_t>(p) + static_cast<size_t>(q) * args.ldc;
+                        if (q < it.q_end) store_c(args, Cb, i, x);
+                        if (q + 1 < it.q_end) store_c(args, Cb, i + args.ldc, y);
+                    }
                 }
             }
         }
+        if (C_::WIDE && lane == 0) bulk_wait_group_all();  // C is written before the kernel ends
     }
 
     __syncwarp();
-    if (CG == 1 && args.split > 1) {
+    if (!C_::WIDE && args.split > 1) {
         cluster_sync();  // every slice's sums are in its CTA's shared memory
         if (item_at<CG, BN>(args, tile_start, off, tile0, rank, it) && !it.bad) {
             const int cols = (BN + args.split - 1) / args.split;
             const int first = static_cast<int>(rank) * cols, last = min(first + cols, BN);
-            void *Cb = args.C;
-            if (args.ragged == GS_GROUP_K)
-                Cb = static_cast<uint8_t *>(args.C) + static_cast<size_t>(it.g) * args.stride_c * (args.out_kind == OUT_F32 ? 4 : 2);
+            void *Cb = group_c(args, it.g);
             for (int e = first * BM + static_cast<int>(threadIdx.x); e < last * BM; e += C_::THREADS) {
-                const int col = it.n0 + e / BM, r = it.m0 + e % BM;
-                if (col >= it.n_end || r >= args.m) continue;
+                const int q = it.q0 + e / BM, p = it.p0 + e % BM;
+                if (q >= it.q_end || p >= it.p_end) continue;
                 float sum = 0.0f;
-                for (int q = 0; q < args.split; ++q)
-                    sum = __fadd_rn(sum, ld_cluster_f32(mapa_shared(smem_u32(smem) + e * 4, static_cast<uint32_t>(q))));
-                store_c(args, Cb, static_cast<size_t>(r) + static_cast<size_t>(col) * args.ldc, sum);
+                for (int x = 0; x < args.split; ++x)
+                    sum = __fadd_rn(sum, ld_cluster_f32(mapa_shared(smem_u32(smem) + e * 4, static_cast<uint32_t>(x))));
+                store_c(args, Cb, static_cast<size_t>(p) + static_cast<size_t>(q) * args.ldc, sum);
             }
         }
         __syncwarp();
@@ -584,6 +723,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         else tmem_dealloc(tmem_base, C_::TMEM_COLS);
     }
 }
+
+struct Maps {
+    CUtensorMap p, q, c;
+};
 
 // CTA pairs that can be resident at once.
 template <int CG, int BN, int MODE>
@@ -611,7 +754,7 @@ static int max_pairs(Context &ctx, size_t smem) {
 }
 
 template <int CG, int BN, int MODE>
-static cudaError_t launch(Context &ctx, const CUtensorMap &ta, const CUtensorMap &tb, const Args &a, long long tiles) {
+static cudaError_t launch(Context &ctx, const Maps &maps, const Args &a, long long tiles) {
     using C_ = Cfg<CG, BN>;
     auto kern = k_gemm_fp8<CG, BN, MODE>;
     constexpr size_t kMost = C_::SMEM + 2 * sizeof(int) * (GS_FP8_MAX_GROUPS + 1);
@@ -628,18 +771,18 @@ static cudaError_t launch(Context &ctx, const CUtensorMap &ta, const CUtensorMap
     long long units = CG == 2 ? max_pairs<CG, BN, MODE>(ctx, kMost) : ctx.sm_count;
     if (CG == 1 && a.split > 1) units = tiles;  // one tile per cluster
     if (tiles < units) units = tiles;
-    e = launch_pdl(kern, dim3(static_cast<unsigned>(units * cluster)), dim3(C_::THREADS), smem, ctx.stream, cluster, ta, tb, a);
+    e = launch_pdl(kern, dim3(static_cast<unsigned>(units * cluster)), dim3(C_::THREADS), smem, ctx.stream, cluster, maps.p, maps.q, maps.c, a);
     ctx.launches++;
     return e;
 }
 
 template <int CG, int BN>
-static cudaError_t launch_mode(Context &ctx, int mode, const CUtensorMap &ta, const CUtensorMap &tb, const Args &a, long long tiles) {
+static cudaError_t launch_mode(Context &ctx, int mode, const Maps &maps, const Args &a, long long tiles) {
     switch (mode) {
-    case 0: return launch<CG, BN, 0>(ctx, ta, tb, a, tiles);
-    case 1: return launch<CG, BN, 1>(ctx, ta, tb, a, tiles);
-    case 2: return launch<CG, BN, 2>(ctx, ta, tb, a, tiles);
-    default: return launch<CG, BN, 3>(ctx, ta, tb, a, tiles);
+    case 0: return launch<CG, BN, 0>(ctx, maps, a, tiles);
+    case 1: return launch<CG, BN, 1>(ctx, maps, a, tiles);
+    case 2: return launch<CG, BN, 2>(ctx, maps, a, tiles);
+    default: return launch<CG, BN, 3>(ctx, maps, a, tiles);
     }
 }
 
@@ -648,11 +791,12 @@ static int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) 
 // Tile of a product: bn columns, cg CTAs, split K slices.
 Tile choose_tile(const GemmFp8Desc &d, int sm_count) {
     Tile t{1, 256, 1};
-    // Columns a tile can expect to fill: a ragged group's mean share, or all of them.
+    // Columns of C a tile can expect to fill: a ragged group's mean share, or all of them.
     const long long cols = d.groups > 0 && d.ragged == GS_GROUP_N ? cdiv(d.n, d.groups) : d.n;
-    if (!d.trans_b) t.bn = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
-    else t.bn = cols <= 128 ? 128 : 256;
-    if (t.bn == 256 && d.m > BM && sm_count >= 2) t.cg = 2;
+    if (cols <= 32 && !d.trans_b) t.bn = 32;
+    else if (cols <= 64 && !d.trans_b) t.bn = 64;
+    else if (cols <= 128) t.bn = 128;
+    else t.cg = sm_count >= 2 ? 2 : 1;
     return t;
 }
 
@@ -661,37 +805,42 @@ Tile choose_tile(const GemmFp8Desc &d, int sm_count) {
 cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     using namespace fp8;
     const Tile t = choose_tile(d, ctx.sm_count);
+    const bool wide = t.bn == 256;
+    const bool ragged_n = d.groups > 0 && d.ragged == GS_GROUP_N, ragged_k = d.groups > 0 && d.ragged == GS_GROUP_K;
+    // A scale matrix per 128 x 128 block is laid out as its operand is; a scale per vector has the non-K index first.
+    Side sa{}, sb{};
+    sa.extent = d.m;
+    sa.mn = d.trans_a ? 0 : 1;
+    sa.grouped = ragged_n && d.groups > 1 && d.stride_a > 0 ? 1 : 0;
+    sa.scale = d.sa;
+    sa.s_i = d.a_vec || !d.trans_a ? 1 : d.ldsa;
+    sa.s_k = d.a_vec || !d.trans_a ? d.ldsa : 1;
+    sa.s_g = ragged_n ? d.stride_sa : 0;
+    sb.extent = d.n;
+    sb.mn = d.trans_b ? 1 : 0;
+    sb.scale = d.sb;
+    sb.s_i = d.b_vec || d.trans_b ? 1 : d.ldsb;
+    sb.s_k = d.b_vec || d.trans_b ? d.ldsb : 1;
     Args a{};
-    a.m = d.m;
-    a.n = d.n;
+    a.p = wide ? sb : sa;
+    a.q = wide ? sa : sb;
     a.k = d.k;
-    a.m_blocks = cdiv(d.m, static_cast<long long>(BM) * t.cg);
-    a.n_blocks = cdiv(d.n, t.bn);
+    a.p_blocks = cdiv(a.p.extent, static_cast<long long>(BM) * t.cg);
+    a.q_blocks = cdiv(a.q.extent, t.bn);
     a.k_blocks = cdiv(d.k, BK);
     a.groups = d.groups;
     a.ragged = d.groups > 0 ? d.ragged : -1;
     a.offsets = d.offsets;
-    a.group_m = a.m_blocks < 8 ? a.m_blocks : 8;
     a.split = t.split;
-    const bool ragged_n = a.groups > 0 && a.ragged == GS_GROUP_N;
     // Ragged N: an upper bound (each group may end in a part tile); the kernel counts the tiles itself.
-    const long long tiles = ragged_n ? static_cast<long long>(a.m_blocks) * (d.n / t.bn + (d.groups < d.n ? d.groups : d.n))
-                                     : static_cast<long long>(a.m_blocks) * a.n_blocks * (a.groups > 0 ? a.groups : 1);
+    const long long tile_n = wide ? BM * t.cg : t.bn, across = wide ? a.q_blocks : a.p_blocks;
+    const long long tiles = ragged_n ? across * (d.n / tile_n + (d.groups < d.n ? d.groups : d.n))
+                                     : static_cast<long long>(a.p_blocks) * a.q_blocks * (ragged_k ? d.groups : 1);
     a.total_tiles = tiles;
-    a.a_mn = d.trans_a ? 0 : 1;
-    a.b_mn = d.trans_b ? 1 : 0;
-    a.a_bcast = ragged_n && d.groups > 1 && d.stride_a > 0 ? 0 : 1;
-    a.idesc = (1u << 4) | (static_cast<uint32_t>(d.a_e5m2) << 7) | (static_cast<uint32_t>(d.b_e5m2) << 10) |
-              (static_cast<uint32_t>(a.a_mn) << 15) | (static_cast<uint32_t>(a.b_mn) << 16) |
-              ((static_cast<uint32_t>(t.bn) >> 3) << 17) | ((static_cast<uint32_t>(BM * t.cg) >> 4) << 24);
-    // A scale matrix per 128 x 128 block is laid out as its operand is; a scale per vector has the non-K index first.
-    a.sa = d.sa;
-    a.sa_i = d.a_vec ? 1 : (d.trans_a ? d.ldsa : 1);
-    a.sa_k = d.a_vec ? d.ldsa : (d.trans_a ? 1 : d.ldsa);
-    a.sa_g = ragged_n ? d.stride_sa : 0;
-    a.sb = d.sb;
-    a.sb_i = d.b_vec ? 1 : (d.trans_b ? 1 : d.ldsb);
-    a.sb_k = d.b_vec ? d.ldsb : (d.trans_b ? d.ldsb : 1);
+    const uint32_t p_e5m2 = wide ? d.b_e5m2 : d.a_e5m2, q_e5m2 = wide ? d.a_e5m2 : d.b_e5m2;
+    a.idesc = (1u << 4) | (p_e5m2 << 7) | (q_e5m2 << 10) | (static_cast<uint32_t>(a.p.mn) << 15) |
+              (static_cast<uint32_t>(a.q.mn) << 16) | ((static_cast<uint32_t>(t.bn) >> 3) << 17) |
+              ((static_cast<uint32_t>(BM * t.cg) >> 4) << 24);
     a.C = d.C;
     a.ldc = d.ldc;
     a.stride_c = d.stride_c;
@@ -699,29 +848,45 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     a.ep = d.ep;
     a.err = ctx.dev_err;
     a.spin_limit = ctx.spin_limit;
+    const size_t es = out_elem_size(d.out_kind);
+    a.vec_c = reinterpret_cast<uintptr_t>(d.C) % 16 == 0 && d.ldc * es % 16 == 0 && (!ragged_k || d.groups == 1 || d.stride_c * es % 16 == 0);
 
-    CUtensorMap ta{}, tb{};
+    Maps maps{};
+    std::string why;
     if (d.k > 0) {
-        std::string why;
         const uint64_t a0 = d.trans_a ? d.k : d.m, a1 = d.trans_a ? d.m : d.k;
-        const uint64_t batch = a.a_bcast ? 1 : static_cast<uint64_t>(d.groups);
-        const uint64_t a2 = batch > 1 ? static_cast<uint64_t>(d.stride_a) : a1 * static_cast<uint64_t>(d.lda);
+        const uint64_t batch = sa.grouped ? static_cast<uint64_t>(d.groups) : 1;
+        const uint64_t a2 = sa.grouped ? static_cast<uint64_t>(d.stride_a) : a1 * static_cast<uint64_t>(d.lda);
         const uint64_t b0 = d.trans_b ? d.n : d.k, b1 = d.trans_b ? d.k : d.n;
-        const uint32_t b_rows = static_cast<uint32_t>(t.bn / t.cg);
-        if (!encode_tmap_3d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, d.A, a0, a1, batch, static_cast<uint64_t>(d.lda), a2, 128, 128, &why) ||
-            !encode_tmap_3d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, d.B, b0, b1, 1, static_cast<uint64_t>(d.ldb),
-                            b1 * static_cast<uint64_t>(d.ldb), 128, d.trans_b ? 128 : b_rows, &why)) {
+        const uint32_t q_box = a.q.mn ? 128 : static_cast<uint32_t>(t.bn / t.cg);
+        if (!encode_tmap_3d(wide ? &maps.q : &maps.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, d.A, a0, a1, batch, static_cast<uint64_t>(d.lda),
+                            a2, 128, wide ? q_box : 128, &why) ||
+            !encode_tmap_3d(wide ? &maps.p : &maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, d.B, b0, b1, 1, static_cast<uint64_t>(d.ldb),
+                            b1 * static_cast<uint64_t>(d.ldb), 128, wide ? 128 : q_box, &why)) {
             ctx.last_error = "tensor map encode failed: " + why;
             return cudaErrorInvalidValue;
         }
     }
-    const int mode = (d.a_vec ? 1 : 0) | (d.b_vec ? 2 : 0);
+    if (wide && a.vec_c && a.ep.beta_zero) {
+        const CUtensorMapDataType dt = d.out_kind == OUT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : d.out_kind == OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const uint64_t row = static_cast<uint64_t>(d.ldc) * es;
+        const bool many = ragged_k && d.groups > 1;
+        a.tma_store = encode_tmap_3d(&maps.c, dt, d.C, d.m, d.n, many ? d.groups : 1, row,
+                                     many ? static_cast<uint64_t>(d.stride_c) * es : row * static_cast<uint64_t>(d.n),
+                                     static_cast<uint32_t>(128 / es), 32, nullptr)
+                          ? 1
+                          : 0;
+    }
+    const bool p_vec = wide ? d.b_vec : d.a_vec, q_vec = wide ? d.a_vec : d.b_vec;
+    const int mode = (p_vec ? 1 : 0) | (q_vec ? 2 : 0);
     ctx.last_kernels |= GS_KERNEL_TC_F8;
-    if (t.cg == 2) return launch_mode<2, 256>(ctx, mode, ta, tb, a, tiles);
-    if (t.bn == 256) return launch_mode<1, 256>(ctx, mode, ta, tb, a, tiles);
-    if (t.bn == 128) return launch_mode<1, 128>(ctx, mode, ta, tb, a, tiles);
-    if (t.bn == 64) return launch_mode<1, 64>(ctx, mode, ta, tb, a, tiles);
-    return launch_mode<1, 32>(ctx, mode, ta, tb, a, tiles);
+    if (t.cg == 2) return launch_mode<2, 256>(ctx, mode, maps, a, tiles);
+    if (t.bn == 256) return launch_mode<1, 256>(ctx, mode, maps, a, tiles);
+    if (t.bn == 128) return launch_mode<1, 128>(ctx, mode, maps, a, tiles);
+    if (t.bn == 64) return launch_mode<1, 64>(ctx, mode, maps, a, tiles);
+    return launch_mode<1, 32>(ctx, mode, maps, a, tiles);
 }
 
 }  // namespace gs
