@@ -225,6 +225,23 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
+// Each thread of the warp reads 16 consecutive 32-bit columns of its TMEM lane.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// Waits for two barriers, both polled once before either is waited for: a poll's latency is paid once.
+__device__ __forceinline__ bool mbar_wait2(uint64_t *b1, uint32_t parity1, uint32_t site1, uint64_t *b2, uint32_t parity2,
+                                           uint32_t site2, uint32_t *err, long long limit) {
+    const bool r1 = mbar_try_wait(smem_u32(b1), parity1), r2 = mbar_try_wait(smem_u32(b2), parity2);
+    if (r1 && r2) return true;
+    return (r1 || mbar_wait(b1, parity1, err, site1, limit)) && (r2 || mbar_wait(b2, parity2, err, site2, limit));
+}
+
 // 4-byte asynchronous copy global -> shared; zeros where `in` is false.
 __device__ __forceinline__ void cp_async_f32(uint32_t dst, const float *src, bool in) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
@@ -437,35 +454,42 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     } else if (warp == 1) {
         // ---------------- MMA issuer (even CTA) ----------------
         if (lane == 0 && leader) {
+            // Descriptors of stage 0; a stage and a K step of 32 only move the address field. The issue loop is one
+            // thread's dependent instructions, and building descriptors in it took longer than the MMAs (815 cycles a
+            // K block without promoters, of which the tensor core worked 512).
+            uint64_t pdesc = umma_smem_desc_sw128(smem_u32(smP), args.p.mn ? 128 * BK : 16, 1024);
+            uint64_t qdesc = umma_smem_desc_sw128(smem_u32(smQ), args.q.mn ? 128 * BK : 16, 1024);
+            const uint32_t p_step = (args.p.mn ? 32 * 128 : 32) >> 4, q_step = (args.q.mn ? 32 * 128 : 32) >> 4;
             int stage = 0, slot = 0;
             uint32_t phase = 0, sphase = 0;
             bool ok = true;
             for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
+#pragma unroll 1
                 for (int kb = 0; kb < it.nkb; ++kb) {
-                    if (!mbar_wait(&tempty[slot], sphase ^ 1u, args.err, 2, args.spin_limit) ||
-                        !mbar_wait(&full[stage], phase, args.err, 3, args.spin_limit)) {
+                    if (!mbar_wait2(&tempty[slot], sphase ^ 1u, 2, &full[stage], phase, 3, args.err, args.spin_limit)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t p_base = smem_u32(smP + stage * C_::P_STAGE);
-                    const uint32_t q_base = smem_u32(smQ + stage * C_::Q_STAGE);
+                    const uint32_t d_tmem = tmem_base + slot * BN;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t pdesc = args.p.mn ? umma_smem_desc_sw128(p_base + kk * 32 * 128, 128 * BK, 1024)
-                                                         : umma_smem_desc_sw128(p_base + kk * 32, 16, 1024);
-                        const uint64_t qdesc = args.q.mn ? umma_smem_desc_sw128(q_base + kk * 32 * 128, 128 * BK, 1024)
-                                                         : umma_smem_desc_sw128(q_base + kk * 32, 16, 1024);
-                        umma_f8<CG>(tmem_base + slot * BN, pdesc, qdesc, args.idesc, kk != 0 ? 1u : 0u);
-                    }
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_f8<CG>(d_tmem, pdesc + kk * p_step, qdesc + kk * q_step, args.idesc, kk != 0 ? 1u : 0u);
                     if constexpr (CG == 2) {
-                        umma_commit_2sm(&empty[stage], 0x3);
                         umma_commit_2sm(&tfull[slot], 0x3);
+                        umma_commit_2sm(&empty[stage], 0x3);
                     } else {
-                        umma_commit(&empty[stage]);
                         umma_commit(&tfull[slot]);
+                        umma_commit(&empty[stage]);
                     }
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    pdesc += C_::P_STAGE >> 4;
+                    qdesc += C_::Q_STAGE >> 4;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                        pdesc -= STAGES * C_::P_STAGE >> 4;
+                        qdesc -= STAGES * C_::Q_STAGE >> 4;
+                    }
                     if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
                 }
             }
@@ -542,27 +566,27 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
 #pragma unroll 1
             for (int kb = 0; kb < it.nkb; ++kb) {
                 // every lane takes the same way out (tcgen05.ld is warp-aligned)
-                if (!__all_sync(0xffffffffu, mbar_wait(&sfull[ss], sp, args.err, 7, args.spin_limit) &&
-                                                 mbar_wait(&tfull[slot], phase, args.err, 4, args.spin_limit))) {
+                if (!__all_sync(0xffffffffu, mbar_wait2(&sfull[ss], sp, 7, &tfull[slot], phase, 4, args.err, args.spin_limit))) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                // The next 32 columns are on their way while these are added.
+                // The next 16 columns are on their way while these are added. (32 at a time spilled the sums: 0.67 instead
+                // of 0.58 us a K block.)
                 const uint32_t t_slot = t_lane + slot * BN + c_lo;
-                uint32_t r[2][32];
-                tmem_ld_32x32b_x32(t_slot, r[0]);
+                uint32_t r[2][16];
+                tmem_ld_x16(t_slot, r[0]);
                 const float *sc = scales + ss * C_::SC_FLOATS;
                 const uint32_t sc_addr = smem_u32(sc + c_lo);
                 float s = sc[BN + (P_VEC ? row : 0)];
                 if constexpr (!Q_VEC) s = __fmul_rn(s, sc[c_lo / 128]);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
-                for (int c = 0; c < EPI_COLS; c += 32) {
-                    const int cur = (c / 32) & 1;
+                for (int c = 0; c < EPI_COLS; c += 16) {
+                    const int cur = (c / 16) & 1;
                     tmem_wait_ld();
-                    if (c + 32 < EPI_COLS) {
-                        tmem_ld_32x32b_x32(t_slot + c + 32, r[cur ^ 1]);
+                    if (c + 16 < EPI_COLS) {
+                        tmem_ld_x16(t_slot + c + 16, r[cur ^ 1]);
                     } else {  // the slot is read: the tensor core may fill it again
                         tc_fence_before();
                         __syncwarp();
@@ -572,7 +596,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
+                    for (int j = 0; j < 16; j += 4) {
                         const uint64_t p0 = pack2(__uint_as_float(r[cur][j]), __uint_as_float(r[cur][j + 1]));
                         const uint64_t p1 = pack2(__uint_as_float(r[cur][j + 2]), __uint_as_float(r[cur][j + 3]));
                         uint64_t &a0 = acc[(c + j) / 2], &a1 = acc[(c + j) / 2 + 1];
