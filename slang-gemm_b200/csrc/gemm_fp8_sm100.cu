@@ -193,19 +193,47 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return d;
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+    return r;
+}
+
+// The MMA and its commits, executed by the whole warp and issued by the lane with `lead` set: with uniform control flow
+// the descriptors stay in uniform registers, where the instruction wants them.
 template <int CG>
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
+                                        uint32_t lead) {
     if constexpr (CG == 2) {
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
-            "r"(idesc), "r"(accumulate)
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
+            "r"(idesc), "r"(accumulate), "r"(lead)
             : "memory");
     } else {
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
-            "r"(idesc), "r"(accumulate)
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
+            "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void umma_commit_lead(uint64_t *bar, uint32_t lead) {
+    if constexpr (CG == 2) {
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(
+                smem_u32(bar)),
+            "h"(static_cast<uint16_t>(3)), "r"(lead)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+            "r"(lead)
             : "memory");
     }
 }
@@ -328,7 +356,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     int *off = reinterpret_cast<int *>(tmem_holder + 2);   // groups + 1 clamped offsets, then groups + 1 first tiles
     int *tile_start = off + args.groups + 1;
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform for the compiler too
     const int lane = threadIdx.x & 31;
     const bool clustered = CG == 2 || args.split > 1;
     const uint32_t rank = clustered ? cluster_ctarank() : 0u;
@@ -453,20 +481,22 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (even CTA) ----------------
-        if (lane == 0 && leader) {
-            // Descriptors of stage 0; a stage and a K step of 32 only move the address field. The issue loop is one
-            // thread's dependent instructions, and building descriptors in it took longer than the MMAs (815 cycles a
-            // K block without promoters, of which the tensor core worked 512).
+        if (leader) {
+            // Descriptors of stage 0; a stage and a K step of 32 only move the address field. The issue loop is a chain of
+            // dependent instructions on a scheduler that two promoters share: with descriptors built in it by one lane
+            // it, and not the tensor core, set the pace (815 cycles a K block without promoters for 512 of MMA).
             uint64_t pdesc = umma_smem_desc_sw128(smem_u32(smP), args.p.mn ? 128 * BK : 16, 1024);
             uint64_t qdesc = umma_smem_desc_sw128(smem_u32(smQ), args.q.mn ? 128 * BK : 16, 1024);
             const uint32_t p_step = (args.p.mn ? 32 * 128 : 32) >> 4, q_step = (args.q.mn ? 32 * 128 : 32) >> 4;
+            const uint32_t lead = elect_one();
             int stage = 0, slot = 0;
             uint32_t phase = 0, sphase = 0;
             bool ok = true;
             for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
 #pragma unroll 1
                 for (int kb = 0; kb < it.nkb; ++kb) {
-                    if (!mbar_wait2(&tempty[slot], sphase ^ 1u, 2, &full[stage], phase, 3, args.err, args.spin_limit)) {
+                    if (!__all_sync(0xffffffffu, mbar_wait2(&tempty[slot], sphase ^ 1u, 2, &full[stage], phase, 3, args.err,
+                                                            args.spin_limit))) {
                         ok = false;
                         break;
                     }
@@ -474,14 +504,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                     const uint32_t d_tmem = tmem_base + slot * BN;
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_f8<CG>(d_tmem, pdesc + kk * p_step, qdesc + kk * q_step, args.idesc, kk != 0 ? 1u : 0u);
-                    if constexpr (CG == 2) {
-                        umma_commit_2sm(&tfull[slot], 0x3);
-                        umma_commit_2sm(&empty[stage], 0x3);
-                    } else {
-                        umma_commit(&tfull[slot]);
-                        umma_commit(&empty[stage]);
-                    }
+                        umma_f8<CG>(d_tmem, pdesc + kk * p_step, qdesc + kk * q_step, args.idesc, kk != 0 ? 1u : 0u, lead);
+                    umma_commit_lead<CG>(&tfull[slot], lead);
+                    umma_commit_lead<CG>(&empty[stage], lead);
                     pdesc += C_::P_STAGE >> 4;
                     qdesc += C_::Q_STAGE >> 4;
                     if (++stage == STAGES) {
@@ -494,8 +519,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                 }
             }
             if (!ok) {  // the MMAs already issued end before the CTA frees its TMEM
-                if constexpr (CG == 2) umma_commit_2sm(drain, 0x3);
-                else umma_commit(drain);
+                umma_commit_lead<CG>(drain, lead);
                 mbar_wait(drain, 0, args.err, 5, args.spin_limit);
             }
         }
