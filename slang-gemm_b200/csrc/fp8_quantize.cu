@@ -18,6 +18,9 @@
 // registers between the maximum and the cast.
 #include <cuda_fp8.h>
 
+#include <cstring>
+#include <type_traits>
+
 #include "gs_float.cuh"
 #include "gs_fp8.h"
 
@@ -63,19 +66,6 @@ __device__ __forceinline__ uint2 cast8(const float (&x)[8], float inv, bool odd)
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight elements from row r of a column (rows past the end read as 0).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *col, int r, int rows, float (&x)[8]) {
-    if (VEC && r + 8 <= rows) {
-        const Pack<T, 8> p = load_pack<T, 8>(col + r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(p.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = r + i < rows ? to_f32(col[r + i]) : 0.0f;
-    }
-}
-
 template <bool VEC>
 __device__ __forceinline__ void store8(uint8_t *col, int r, int rows, uint2 q) {
     if (VEC && r + 8 <= rows) {
@@ -99,44 +89,108 @@ __device__ __forceinline__ const T *source(const QuantDesc &d, int c) {
     return s < 0 ? nullptr : static_cast<const T *>(d.src) + s * d.ld_src;
 }
 
-// Vectors down the columns: 16 lanes hold one vector of 128 rows.
+// amax as f32 bits of eight raw elements: of all of them, or (second time, where that is not finite) of the finite ones.
+__device__ __forceinline__ uint32_t top_bits(const Pack<float, 8> &p, bool finite) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = abs_bits(p.v[i]);
+        top = max(top, finite && b >= kInf ? 0u : b);
+    }
+    return top;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Pack<T, 8> &p, bool finite) {  // 16-bit types: two at a time, as integers
+    static_assert(sizeof(T) == 2, "two elements to a word");
+    constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&p);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t b = w[i] & 0x7fff7fffu;
+        if (finite) {
+            if ((b & 0xffffu) >= inf) b &= 0xffff0000u;
+            if ((b >> 16) >= inf) b &= 0xffffu;
+        }
+        top = __vmaxu2(top, b);
+    }
+    T v;
+    const uint16_t h = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    memcpy(&v, &h, 2);
+    return __float_as_uint(to_f32(v));
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ Pack<T, 8> load_raw(const T *col, int r, int rows) {
+    Pack<T, 8> p;
+    if (VEC && r + 8 <= rows) {
+        p = load_pack<T, 8>(col + r);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p.v[i] = r + i < rows ? col[r + i] : from_f32<T>(0.0f);
+    }
+    return p;
+}
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> zero_raw() {
+    Pack<T, 8> p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.v[i] = from_f32<T>(0.0f);
+    return p;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Pack<T, 8> &p, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(p.v[i]);
+}
+
+// Vectors down the columns: 16 lanes hold one vector of 128 rows. `lanes` (16 to 256) threads of a block take a
+// column, DEPTH vectors of each thread's on their way at once.
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(256) k_quant_down(const QuantDesc d) {
+__global__ void __launch_bounds__(256) k_quant_down(const QuantDesc d, int lanes) {
+    constexpr int DEPTH = sizeof(T) == 4 ? 2 : 4;
     grid_dep_wait();
     grid_dep_launch();
-    const int rb_n = (d.rows + 127) / 128;
-    const long long tasks = static_cast<long long>(rb_n) * d.cols;
-    const int sub = threadIdx.x & 15;
+    const int sub = threadIdx.x & 15, per = 256 / lanes;  // columns a block takes at once
     const uint32_t half = 0xffffu << (threadIdx.x & 16);
-    for (long long task = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / 16; task < tasks; task += static_cast<long long>(gridDim.x) * 16) {
-        const int c = static_cast<int>(task / rb_n), rb = static_cast<int>(task - static_cast<long long>(c) * rb_n);
-        const int r = rb * 128 + sub * 8;
-        const T *src = source<T>(d, c);
-        float x[8] = {};
-        if (src != nullptr) load8<T, VEC>(src, r, d.rows, x);
-        uint32_t top = 0;
+    for (long long c = static_cast<long long>(blockIdx.x) * per + threadIdx.x / lanes; c < d.cols; c += static_cast<long long>(gridDim.x) * per) {
+        const T *src = source<T>(d, static_cast<int>(c));
+        uint8_t *dst = static_cast<uint8_t *>(d.dst) + c * d.ld_dst;
+        const int first = (threadIdx.x % lanes) * 8, step = lanes * 8;
+        for (int r0 = first; r0 - sub * 8 < d.rows; r0 += DEPTH * step) {
+            Pack<T, 8> raw[DEPTH];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(x[i]));
+            for (int i = 0; i < DEPTH; ++i) {
+                const int r = r0 + i * step;
+                raw[i] = src != nullptr && r < d.rows ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
+            }
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
-        const bool odd = top >= kInf;
-        if (odd) {  // the same answer in all 16 lanes
-            top = 0;
+            for (int i = 0; i < DEPTH; ++i) {
+                const int r = r0 + i * step;
+                if (r - sub * 8 >= d.rows) break;  // the same answer in all 16 lanes
+                uint32_t top = top_bits(raw[i], false);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, abs_bits(x[i]) < kInf ? abs_bits(x[i]) : 0u);
+                for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
+                const bool odd = top >= kInf;
+                if (odd) {
+                    top = top_bits(raw[i], true);
 #pragma unroll
-            for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
+                    for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
+                }
+                const int e = scale_exp<E5M2>(top);
+                if (sub == 0) d.scale[c + (r / 128) * d.ld_scale] = pow2(e);
+                float x[8];
+                widen(raw[i], x);
+                if (r < d.rows) store8<VEC>(dst, r, d.rows, cast8<E5M2>(x, pow2(-e), odd));
+            }
         }
-        const int e = scale_exp<E5M2>(top);
-        if (sub == 0) d.scale[c + rb * d.ld_scale] = pow2(e);
-        store8<VEC>(static_cast<uint8_t *>(d.dst) + c * d.ld_dst, r, d.rows, cast8<E5M2>(x, pow2(-e), odd));
     }
 }
 
 // Tiles of 128 columns: vectors along the rows (BLK false, 64 rows a tile) or
-// 128 x 128 blocks. A thread holds 8 rows of COLS columns.
+// 128 x 128 blocks. A thread holds 8 rows of COLS columns, as they were loaded.
 template <typename T, bool E5M2, bool VEC, bool BLK>
-__global__ void __launch_bounds__(256) k_quant_tile(const QuantDesc d) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_tile(const QuantDesc d) {
     constexpr int ROWS = BLK ? 128 : 64, LANES = ROWS / 8, STEP = 256 / LANES, COLS = 128 / STEP;
     __shared__ uint32_t red[8][ROWS];
     grid_dep_wait();
@@ -147,37 +201,47 @@ __global__ void __launch_bounds__(256) k_quant_tile(const QuantDesc d) {
     for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
         const int ct = static_cast<int>(task / rt_n), rt = static_cast<int>(task - static_cast<long long>(ct) * rt_n);
         const int r = rt * ROWS + lr * 8;
-        float x[COLS][8] = {};
+        Pack<T, 8> x[COLS];
+        // Whole tiles load without a branch between the loads, so that all of them are on their way at once.
+        const bool whole = VEC && d.index == nullptr && (rt + 1) * ROWS <= d.rows && (ct + 1) * 128 <= d.cols;
+        if (whole) {
+            const T *src = static_cast<const T *>(d.src) + (static_cast<long long>(ct) * 128 + lc) * d.ld_src + r;
 #pragma unroll
-        for (int i = 0; i < COLS; ++i) {
-            const int c = ct * 128 + lc + i * STEP;
-            const T *src = c < d.cols ? source<T>(d, c) : nullptr;
-            if (src != nullptr) load8<T, VEC>(src, r, d.rows, x[i]);
+            for (int i = 0; i < COLS; ++i) x[i] = load_pack<T, 8>(src + static_cast<long long>(i * STEP) * d.ld_src);
+        } else {
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) {
+                const int c = ct * 128 + lc + i * STEP;
+                const T *src = c < d.cols ? source<T>(d, c) : nullptr;
+                x[i] = src != nullptr ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
+            }
         }
-        uint32_t top[8];
+        uint32_t top[BLK ? 1 : 8];
         bool odd = false;
         for (int pass = 0; pass < 2; ++pass) {  // a second time over the finite values, if there are others
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top[j] = 0;
-#pragma unroll
-            for (int i = 0; i < COLS; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t b = abs_bits(x[i][j]);
-                    top[j] = max(top[j], pass == 1 && b >= kInf ? 0u : b);
-                }
             if constexpr (BLK) {
-                uint32_t t = 0;
+                uint32_t m = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t = max(t, top[j]);
-                t = __reduce_max_sync(0xffffffffu, t);
-                if ((threadIdx.x & 31) == 0) red[warp][0] = t;
+                for (int i = 0; i < COLS; ++i) m = max(m, top_bits(x[i], pass == 1));
+                m = __reduce_max_sync(0xffffffffu, m);
+                if ((threadIdx.x & 31) == 0) red[warp][0] = m;
                 __syncthreads();
 #pragma unroll
-                for (int w = 0; w < 8; ++w) t = max(t, red[w][0]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top[j] = t;
+                for (int w = 0; w < 8; ++w) m = max(m, red[w][0]);
+                top[0] = m;
             } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top[j] = 0;
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) {
+                    float v[8];
+                    widen(x[i], v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t b = abs_bits(v[j]);
+                        top[j] = max(top[j], pass == 1 && b >= kInf ? 0u : b);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
@@ -192,52 +256,45 @@ __global__ void __launch_bounds__(256) k_quant_tile(const QuantDesc d) {
             }
             bool any = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) any |= top[j] >= kInf;
+            for (int j = 0; j < (BLK ? 1 : 8); ++j) any |= top[j] >= kInf;
             if (!__syncthreads_or(any)) break;
             odd = true;
         }
-        if constexpr (BLK) {
-            const int e = scale_exp<E5M2>(top[0]);
-            if (threadIdx.x == 0) d.scale[rt + ct * d.ld_scale] = pow2(e);
-            const float inv = pow2(-e);
+        float inv[BLK ? 1 : 8];
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) {
-                const int c = ct * 128 + lc + i * STEP;
-                if (c < d.cols)
-                    store8<VEC>(static_cast<uint8_t *>(d.dst) + c * d.ld_dst, r, d.rows, cast8<E5M2>(x[i], inv, odd));
-            }
-        } else {
-            float inv[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int e = scale_exp<E5M2>(top[j]);
-                inv[j] = pow2(-e);
+        for (int j = 0; j < (BLK ? 1 : 8); ++j) {
+            const int e = scale_exp<E5M2>(top[j]);
+            inv[j] = pow2(-e);
+            if constexpr (BLK) {
+                if (threadIdx.x == 0) d.scale[rt + ct * d.ld_scale] = pow2(e);
+            } else {
                 if (lc == 0 && r + j < d.rows) d.scale[r + j + ct * d.ld_scale] = pow2(e);
             }
+        }
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) {
-                const int c = ct * 128 + lc + i * STEP;
-                if (c >= d.cols) continue;
-                float y[8];
+        for (int i = 0; i < COLS; ++i) {
+            const int c = ct * 128 + lc + i * STEP;
+            if (c >= d.cols) continue;
+            float y[8];
+            widen(x[i], y);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[i][j], inv[j]);  // keeps NaN and infinity
-                store8<VEC>(static_cast<uint8_t *>(d.dst) + c * d.ld_dst, r, d.rows, cast8<E5M2>(y, 1.0f, odd));
-            }
+            for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(y[j], inv[BLK ? 0 : j]);  // keeps NaN and infinity
+            store8<VEC>(static_cast<uint8_t *>(d.dst) + static_cast<long long>(c) * d.ld_dst, r, d.rows, cast8<E5M2>(y, 1.0f, odd));
         }
     }
 }
 
 template <typename T, bool E5M2, bool VEC>
 static cudaError_t launch(Context &ctx, const QuantDesc &d) {
-    const long long most = 16LL * ctx.sm_count;
-    long long blocks;
     cudaError_t e;
     if (!d.blk && d.axis == 0) {
-        blocks = (static_cast<long long>((d.rows + 127) / 128) * d.cols + 15) / 16;
-        e = launch_pdl(k_quant_down<T, E5M2, VEC>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d);
+        int lanes = 16;
+        while (lanes < 256 && lanes * 8 < d.rows) lanes *= 2;
+        const long long blocks = (static_cast<long long>(d.cols) * lanes + 255) / 256, most = 64LL * ctx.sm_count;
+        e = launch_pdl(k_quant_down<T, E5M2, VEC>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d, lanes);
     } else {
         const int rows = d.blk ? 128 : 64;
-        blocks = static_cast<long long>((d.rows + rows - 1) / rows) * ((d.cols + 127) / 128);
+        const long long blocks = static_cast<long long>((d.rows + rows - 1) / rows) * ((d.cols + 127) / 128), most = 64LL * ctx.sm_count;
         auto kern = d.blk ? k_quant_tile<T, E5M2, VEC, true> : k_quant_tile<T, E5M2, VEC, false>;
         e = launch_pdl(kern, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d);
     }

@@ -40,27 +40,48 @@ __device__ __forceinline__ void store8(T *p, int h, int hidden, const float (&x)
     }
 }
 
-// A thread sums V columns of one token.
+// A thread sums V columns of one token; the token's rows and weights are read first, then up to four of its rows'
+// columns are on their way at once.
 template <typename T, typename TO, bool VEC>
-__global__ void __launch_bounds__(256) k_combine(const CombineDesc d) {
+__global__ void __launch_bounds__(256) k_combine(const CombineDesc d, int lanes) {
     grid_dep_wait();
     grid_dep_launch();
-    const int chunks = (d.hidden + V - 1) / V;
-    const long long tasks = static_cast<long long>(d.tokens) * chunks;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < tasks; i += static_cast<long long>(gridDim.x) * 256) {
-        const long long t = i / chunks;
-        const int h = static_cast<int>(i - t * chunks) * V;
+    const int per = 256 / lanes;  // tokens a block takes at once
+    const int chunks = (d.hidden + V - 1) / V, splits = (chunks + lanes - 1) / lanes;
+    const long long tasks = (static_cast<long long>(d.tokens) + per - 1) / per * splits;
+    for (long long i = blockIdx.x; i < tasks; i += gridDim.x) {
+        const long long t = i / splits * per + threadIdx.x / lanes;
+        const int h = (static_cast<int>(i % splits) * lanes + threadIdx.x % lanes) * V;
+        if (t >= d.tokens || h >= d.hidden) continue;
+        const int32_t *rows = d.slot_row + t * d.top_k;
+        const float *weights = d.weights != nullptr ? d.weights + t * d.top_k : nullptr;
         float sum[V] = {};
-#pragma unroll 4
-        for (int j = 0; j < d.top_k; ++j) {
-            const long long at = t * d.top_k + j;
-            const int r = d.slot_row[at];
-            if (r < 0 || r >= d.rows) continue;
-            const float w = d.weights != nullptr ? d.weights[at] : 1.0f;
-            float x[V];
-            load8<T, VEC>(static_cast<const T *>(d.y) + r * d.ldy, h, d.hidden, x);
+        for (int j = 0; j < d.top_k; j += 4) {
+            int r[4];
+            float w[4], x[4][V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) sum[v] = fmaf(w, x[v], sum[v]);
+            for (int q = 0; q < 4; ++q) {
+                r[q] = j + q < d.top_k ? rows[j + q] : -1;
+                if (r[q] >= d.rows) r[q] = -1;
+                w[q] = weights != nullptr && r[q] >= 0 ? weights[j + q] : 1.0f;
+            }
+            if (VEC && h + V <= d.hidden && min(min(r[0], r[1]), min(r[2], r[3])) >= 0) {  // the usual case, without a branch between the loads
+                Pack<T, V> raw[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) raw[q] = load_pack<T, V>(static_cast<const T *>(d.y) + r[q] * d.ldy + h);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) sum[v] = fmaf(w[q], to_f32(raw[q].v[v]), sum[v]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (r[q] < 0) continue;
+                    load8<T, VEC>(static_cast<const T *>(d.y) + r[q] * d.ldy, h, d.hidden, x[q]);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) sum[v] = fmaf(w[q], x[q][v], sum[v]);
+                }
+            }
         }
         store8<TO, VEC>(static_cast<TO *>(d.out) + t * d.ldo, h, d.hidden, sum);
     }
@@ -120,8 +141,11 @@ static bool aligned(const void *p, long long ld, size_t es) { return reinterpret
 
 cudaError_t launch_combine(Context &ctx, const CombineDesc &d) {
     ctx.last_kernels |= GS_KERNEL_COMBINE;
-    const long long tasks = static_cast<long long>(d.tokens) * ((d.hidden + combine::V - 1) / combine::V);
-    const long long want = (tasks + 255) / 256, most = 32LL * ctx.sm_count;
+    const int chunks = (d.hidden - 1) / combine::V + 1;
+    int lanes = 32;  // threads to a token
+    while (lanes < 256 && lanes < chunks) lanes *= 2;
+    const int per = 256 / lanes;
+    const long long want = (static_cast<long long>(d.tokens) + per - 1) / per * ((chunks + lanes - 1) / lanes), most = 64LL * ctx.sm_count;
     const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
     return with_float_type(d.type, [&](auto z) {
         return with_float_type(d.out_type, [&](auto zo) {
@@ -129,7 +153,7 @@ cudaError_t launch_combine(Context &ctx, const CombineDesc &d) {
             using TO = decltype(zo);
             const bool vec = combine::aligned(d.y, d.ldy, sizeof(T)) && combine::aligned(d.out, d.ldo, sizeof(TO));
             const cudaError_t e = launch_pdl(vec ? combine::k_combine<T, TO, true> : combine::k_combine<T, TO, false>, dim3(blocks),
-                                             dim3(256), 0, ctx.stream, 1, d);
+                                             dim3(256), 0, ctx.stream, 1, d, lanes);
             ctx.launches++;
             return e;
         });
