@@ -44,26 +44,6 @@ __device__ __forceinline__ uint32_t cast2(float x, float y) {
     return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 
-// Eight values times 2^-e as FP8 bytes. `odd`: the block holds a value that is not finite.
-template <bool E5M2>
-__device__ __forceinline__ uint2 cast8(const float (&x)[8], float inv, bool odd) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = cast2<E5M2>(__fmul_rn(x[2 * i], inv), __fmul_rn(x[2 * i + 1], inv));
-    if (odd) {  // the conversion saturates infinities: put E4M3's NaN or E5M2's infinity in their places
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __float_as_uint(x[i]);
-            if ((b & 0x7fffffffu) == kInf) {
-                const uint32_t q = ((b >> 24) & 0x80u) | (E5M2 ? 0x7cu : 0x7fu);
-                const int s = 8 * (i & 1);
-                w[i / 2] = (w[i / 2] & ~(0xffu << s)) | (q << s);
-            }
-        }
-    }
-    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-}
-
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 template <bool VEC>
@@ -89,65 +69,145 @@ __device__ __forceinline__ const T *source(const QuantDesc &d, int c) {
     return s < 0 ? nullptr : static_cast<const T *>(d.src) + s * d.ld_src;
 }
 
-// amax as f32 bits of eight raw elements: of all of them, or (second time, where that is not finite) of the finite ones.
-__device__ __forceinline__ uint32_t top_bits(const Pack<float, 8> &p, bool finite) {
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw {
+    uint4 w[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T> &p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[4 * i] = __uint_as_float(p.w[i].x);
+            x[4 * i + 1] = __uint_as_float(p.w[i].y);
+            x[4 * i + 2] = __uint_as_float(p.w[i].z);
+            x[4 * i + 3] = __uint_as_float(p.w[i].w);
+        }
+    } else {
+        const uint32_t w[4] = {p.w[0].x, p.w[0].y, p.w[0].z, p.w[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            }
+        }
+    }
+}
+
+// Bits of the largest |x| of eight raw elements as f32. NaN is passed over (all eight NaN: NaN), an infinity is not:
+// at or above kInf, ask again with finite_top.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Raw<T> &p) {
+    if constexpr (sizeof(T) == 4) {
+        float x[8];
+        widen(p, x);
+        float top = fabsf(x[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        return abs_bits(top);
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const uint32_t w[4] = {p.w[0].x, p.w[0].y, p.w[0].z, p.w[0].w};
+        T2 m = __habs2(*reinterpret_cast<const T2 *>(&w[0]));
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const T2 *>(&w[i])));
+        const uint32_t b = *reinterpret_cast<const uint32_t *>(&m);
+        if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(m);
+            return abs_bits(fmaxf(f.x, f.y));
+        } else {
+            return max(b << 16, b & 0xffff0000u);
+        }
+    }
+}
+// Cold: blocks that hold values that are not finite.
+template <typename T>
+__device__ __noinline__ uint32_t finite_top(const Raw<T> p) {
+    float x[8];
+    widen(p, x);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t b = abs_bits(p.v[i]);
-        top = max(top, finite && b >= kInf ? 0u : b);
+        const uint32_t b = abs_bits(x[i]);
+        top = max(top, b < kInf ? b : 0u);
     }
     return top;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t top_bits(const Pack<T, 8> &p, bool finite) {  // 16-bit types: two at a time, as integers
-    static_assert(sizeof(T) == 2, "two elements to a word");
-    constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    const uint32_t *w = reinterpret_cast<const uint32_t *>(&p);
-    uint32_t top = 0;
+// The conversion saturates infinities: puts E4M3's NaN or E5M2's infinity in their places.
+template <typename T, bool E5M2>
+__device__ __noinline__ uint2 mend_infinities(const Raw<T> p, uint2 q) {
+    float x[8];
+    widen(p, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t b = w[i] & 0x7fff7fffu;
-        if (finite) {
-            if ((b & 0xffffu) >= inf) b &= 0xffff0000u;
-            if ((b >> 16) >= inf) b &= 0xffffu;
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(x[i]);
+        if ((b & 0x7fffffffu) == kInf) {
+            const uint32_t v = ((b >> 24) & 0x80u) | (E5M2 ? 0x7cu : 0x7fu);
+            const int s = 8 * (i & 3);
+            uint32_t &w = i < 4 ? q.x : q.y;
+            w = (w & ~(0xffu << s)) | (v << s);
         }
-        top = __vmaxu2(top, b);
     }
-    T v;
-    const uint16_t h = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
-    memcpy(&v, &h, 2);
-    return __float_as_uint(to_f32(v));
+    return q;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Pack<T, 8> load_raw(const T *col, int r, int rows) {
-    Pack<T, 8> p;
-    if (VEC && r + 8 <= rows) {
-        p = load_pack<T, 8>(col + r);
-    } else {
+// Eight raw elements times inv[0..7] (or inv[0]) as FP8 bytes. `odd`: there may be infinities among them.
+template <typename T, bool E5M2, int N>
+__device__ __forceinline__ uint2 cast8(const Raw<T> &p, const float (&inv)[N], bool odd) {
+    float x[8];
+    widen(p, x);
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p.v[i] = r + i < rows ? col[r + i] : from_f32<T>(0.0f);
+    for (int i = 0; i < 4; ++i) {
+        const float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(inv[(2 * i) % N], inv[(2 * i + 1) % N]));
+        w[i] = cast2<E5M2>(y.x, y.y);
     }
+    uint2 q = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+    if (odd) q = mend_infinities<T, E5M2>(p, q);
+    return q;
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> zero_raw() {
+    Raw<T> p;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) p.w[i] = make_uint4(0, 0, 0, 0);
     return p;
 }
 template <typename T>
-__device__ __forceinline__ Pack<T, 8> zero_raw() {
-    Pack<T, 8> p;
+__device__ __forceinline__ Raw<T> load_whole(const T *p) {
+    Raw<T> q;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p.v[i] = from_f32<T>(0.0f);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) q.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return q;
+}
+// Element by element: the edge of the matrix, and addresses that are not multiples of 16 bytes.
+template <typename T>
+__device__ __noinline__ Raw<T> load_part(const T *col, int r, int rows) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r + i < rows ? col[r + i] : from_f32<T>(0.0f);
+    Raw<T> p;
+    memcpy(&p, v, sizeof(p));
     return p;
 }
-template <typename T>
-__device__ __forceinline__ void widen(const Pack<T, 8> &p, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(p.v[i]);
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw<T> load_raw(const T *col, int r, int rows) {
+    if (VEC && r + 8 <= rows) return load_whole<T>(col + r);
+    return load_part<T>(col, r, rows);
 }
 
 // Vectors down the columns: 16 lanes hold one vector of 128 rows. `lanes` (16 to 256) threads of a block take a
 // column, DEPTH vectors of each thread's on their way at once.
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(256) k_quant_down(const QuantDesc d, int lanes) {
+__global__ void __launch_bounds__(256, 5) k_quant_down(const QuantDesc d, int lanes) {
     constexpr int DEPTH = sizeof(T) == 4 ? 2 : 4;
     grid_dep_wait();
     grid_dep_launch();
@@ -157,31 +217,42 @@ __global__ void __launch_bounds__(256) k_quant_down(const QuantDesc d, int lanes
         const T *src = source<T>(d, static_cast<int>(c));
         uint8_t *dst = static_cast<uint8_t *>(d.dst) + c * d.ld_dst;
         const int first = (threadIdx.x % lanes) * 8, step = lanes * 8;
+        float *sc = d.scale + c + static_cast<long long>(first / 128) * d.ld_scale;
+        const long long sc_step = static_cast<long long>(step / 128) * d.ld_scale;
         for (int r0 = first; r0 - sub * 8 < d.rows; r0 += DEPTH * step) {
-            Pack<T, 8> raw[DEPTH];
+            Raw<T> raw[DEPTH];
+            // Whole vectors in all steps: no branch between the loads.
+            const bool whole = VEC && src != nullptr && r0 - sub * 8 + (DEPTH - 1) * step + 128 <= d.rows;
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < DEPTH; ++i) {
-                const int r = r0 + i * step;
-                raw[i] = src != nullptr && r < d.rows ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
+                for (int i = 0; i < DEPTH; ++i) raw[i] = load_whole<T>(src + r0 + i * step);
+            } else {
+#pragma unroll
+                for (int i = 0; i < DEPTH; ++i) {
+                    const int r = r0 + i * step;
+                    raw[i] = src != nullptr && r < d.rows ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
+                }
             }
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i) {
                 const int r = r0 + i * step;
-                if (r - sub * 8 >= d.rows) break;  // the same answer in all 16 lanes
-                uint32_t top = top_bits(raw[i], false);
+                if (!whole && r - sub * 8 >= d.rows) break;  // the same answer in all 16 lanes
+                uint32_t top = top_bits(raw[i]);
 #pragma unroll
                 for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
                 const bool odd = top >= kInf;
                 if (odd) {
-                    top = top_bits(raw[i], true);
+                    top = finite_top(raw[i]);
 #pragma unroll
                     for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
                 }
                 const int e = scale_exp<E5M2>(top);
-                if (sub == 0) d.scale[c + (r / 128) * d.ld_scale] = pow2(e);
-                float x[8];
-                widen(raw[i], x);
-                if (r < d.rows) store8<VEC>(dst, r, d.rows, cast8<E5M2>(x, pow2(-e), odd));
+                if (sub == 0) *sc = pow2(e);
+                sc += sc_step;
+                const float inv[1] = {pow2(-e)};
+                const uint2 q = cast8<T, E5M2>(raw[i], inv, odd);
+                if (whole) *reinterpret_cast<uint2 *>(dst + r) = q;
+                else if (r < d.rows) store8<VEC>(dst, r, d.rows, q);
             }
         }
     }
@@ -201,13 +272,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_ti
     for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
         const int ct = static_cast<int>(task / rt_n), rt = static_cast<int>(task - static_cast<long long>(ct) * rt_n);
         const int r = rt * ROWS + lr * 8;
-        Pack<T, 8> x[COLS];
+        Raw<T> x[COLS];
         // Whole tiles load without a branch between the loads, so that all of them are on their way at once.
         const bool whole = VEC && d.index == nullptr && (rt + 1) * ROWS <= d.rows && (ct + 1) * 128 <= d.cols;
         if (whole) {
             const T *src = static_cast<const T *>(d.src) + (static_cast<long long>(ct) * 128 + lc) * d.ld_src + r;
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) x[i] = load_pack<T, 8>(src + static_cast<long long>(i * STEP) * d.ld_src);
+            for (int i = 0; i < COLS; ++i) x[i] = load_whole<T>(src + static_cast<long long>(i * STEP) * d.ld_src);
         } else {
 #pragma unroll
             for (int i = 0; i < COLS; ++i) {
@@ -222,7 +293,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_ti
             if constexpr (BLK) {
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) m = max(m, top_bits(x[i], pass == 1));
+                for (int i = 0; i < COLS; ++i) m = max(m, pass == 0 ? top_bits(x[i]) : finite_top(x[i]));
                 m = __reduce_max_sync(0xffffffffu, m);
                 if ((threadIdx.x & 31) == 0) red[warp][0] = m;
                 __syncthreads();
@@ -271,15 +342,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_ti
                 if (lc == 0 && r + j < d.rows) d.scale[r + j + ct * d.ld_scale] = pow2(e);
             }
         }
+        uint8_t *dst = static_cast<uint8_t *>(d.dst) + (static_cast<long long>(ct) * 128 + lc) * d.ld_dst;
 #pragma unroll
         for (int i = 0; i < COLS; ++i) {
-            const int c = ct * 128 + lc + i * STEP;
-            if (c >= d.cols) continue;
-            float y[8];
-            widen(x[i], y);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(y[j], inv[BLK ? 0 : j]);  // keeps NaN and infinity
-            store8<VEC>(static_cast<uint8_t *>(d.dst) + static_cast<long long>(c) * d.ld_dst, r, d.rows, cast8<E5M2>(y, 1.0f, odd));
+            const uint2 q = cast8<T, E5M2>(x[i], inv, odd);
+            uint8_t *col = dst + static_cast<long long>(i * STEP) * d.ld_dst;
+            if (whole) *reinterpret_cast<uint2 *>(col + r) = q;
+            else if (ct * 128 + lc + i * STEP < d.cols) store8<VEC>(col, r, d.rows, q);
         }
     }
 }
@@ -288,8 +357,9 @@ template <typename T, bool E5M2, bool VEC>
 static cudaError_t launch(Context &ctx, const QuantDesc &d) {
     cudaError_t e;
     if (!d.blk && d.axis == 0) {
+        const int depth = sizeof(T) == 4 ? 2 : 4;  // vectors a thread has on their way at once
         int lanes = 16;
-        while (lanes < 256 && lanes * 8 < d.rows) lanes *= 2;
+        while (lanes < 256 && lanes * 8 * depth < d.rows) lanes *= 2;
         const long long blocks = (static_cast<long long>(d.cols) * lanes + 255) / 256, most = 64LL * ctx.sm_count;
         e = launch_pdl(k_quant_down<T, E5M2, VEC>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d, lanes);
     } else {
