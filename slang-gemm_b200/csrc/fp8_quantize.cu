@@ -261,9 +261,10 @@ __global__ void __launch_bounds__(256, 5) k_quant_down(const QuantDesc d, int la
 // Tiles of 128 columns: vectors along the rows (BLK false, 64 rows a tile) or
 // 128 x 128 blocks. A thread holds 8 rows of COLS columns, as they were loaded.
 template <typename T, bool E5M2, bool VEC, bool BLK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_tile(const QuantDesc d) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) k_quant_tile(const QuantDesc d) {
     constexpr int ROWS = BLK ? 128 : 64, LANES = ROWS / 8, STEP = 256 / LANES, COLS = 128 / STEP;
     __shared__ uint32_t red[8][ROWS];
+    __shared__ __align__(16) uint32_t all[ROWS];
     grid_dep_wait();
     grid_dep_launch();
     const int rt_n = (d.rows + ROWS - 1) / ROWS, ct_n = (d.cols + 127) / 128;
@@ -320,10 +321,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && BLK ? 2 : 3) k_quant_ti
                     if ((threadIdx.x & 31) < 8) red[warp][lr * 8 + j] = top[j];
                 }
                 __syncthreads();
+                if (threadIdx.x < ROWS) {
+                    uint32_t m = red[0][threadIdx.x];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int w = 0; w < 8; ++w) top[j] = max(top[j], red[w][lr * 8 + j]);
+                    for (int w = 1; w < 8; ++w) m = max(m, red[w][threadIdx.x]);
+                    all[threadIdx.x] = m;
+                }
+                __syncthreads();
+                const uint4 lo = *reinterpret_cast<const uint4 *>(all + lr * 8), hi = *reinterpret_cast<const uint4 *>(all + lr * 8 + 4);
+                top[0] = lo.x; top[1] = lo.y; top[2] = lo.z; top[3] = lo.w;
+                top[4] = hi.x; top[5] = hi.y; top[6] = hi.z; top[7] = hi.w;
             }
             bool any = false;
 #pragma unroll

@@ -29,6 +29,7 @@ namespace route {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kChooseThreads = 1024;  // of the kernel that only chooses: 32 warps hide the reductions' latency
 constexpr uint32_t kFull = 0xffffffffu;
 
 // Order-preserving keys. -0 and 0 are one value.
@@ -75,18 +76,21 @@ __device__ __forceinline__ void load_row(const T *row, int experts, int lane, fl
     }
 }
 
-// Scores of all experts (masked ones: 0).
+template <int VPL>
+__device__ __forceinline__ float row_top(const float (&l)[VPL]) {
+    float top = l[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) top = fmaxf(top, l[i]);
+    return value_of(warp_max(key_of(top)));
+}
+// Scores of all experts (masked ones: 0). top: softmax's largest logit.
 template <typename R, int VPL>
-__device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, R (&s)[VPL]) {
+__device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, float top, R (&s)[VPL]) {
     if (sigmoid) {
 #pragma unroll
         for (int i = 0; i < VPL; ++i) s[i] = R(1) / (R(1) + exp_of(-R(l[i])));  // -inf: 1 / inf = 0
         return;
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
-    top = value_of(warp_max(key_of(top)));
     R sum = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -94,99 +98,146 @@ __device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, R (&
         sum += s[i];
     }
     sum = warp_sum(sum);
+    const R inv = sum > R(0) ? R(1) / sum : R(0);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) s[i] = sum > R(0) ? s[i] / sum : R(0);
+    for (int i = 0; i < VPL; ++i) s[i] *= inv;
 }
 
-// Chooses a token's experts: lane j < top_k gets the j-th id and its score.
-// Returns false if f32 values that decide something are too close to call.
+// Two best keys of the warp, from each lane's two best.
+template <typename Key>
+__device__ __forceinline__ void warp_top2(Key a1, Key a2, int lane, Key &m1, Key &m2) {
+    m1 = warp_max(a1);
+    const int owner = __ffs(__ballot_sync(kFull, a1 == m1)) - 1;
+    m2 = warp_max(lane == owner ? a2 : a1);
+}
+
+// Chooses a token's experts: lane j < top_k gets the j-th id, or -1. Returns false if f32 values that decide something
+// are too close to call.
 template <typename R, int VPL>
-__device__ bool choose(const RouteDesc &d, const float (&l)[VPL], int lane, int &id, R &score) {
+__device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL], float top, int lane, int &id) {
     using Key = decltype(key_of(R(0)));
     constexpr bool F32 = std::is_same<R, float>::value;
     const Key none = key_of(R(-INFINITY));
-    R s[VPL];
-    scores<R, VPL>(l, d.sigmoid != 0, s);
+    const bool grouped = d.groups > 1 && d.top_groups < d.groups;
     Key key[VPL];
     bool close = false;
     // f32 error of a score, at most 1, and of its sum with the bias
     auto far = [](float x, float y) { return !(fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x)); };
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        if (d.bias != nullptr) {
-            const int e = i * 32 + lane;
-            const R c = e < d.experts ? s[i] + R(d.bias[e]) : R(-INFINITY);
-            key[i] = l[i] == -INFINITY || !(c > R(-INFINITY)) ? none : key_of(c);
-        } else {
-            key[i] = key_of(R(l[i]));
-        }
-    }
-    if (d.groups > 1 && d.top_groups < d.groups) {
-        const int size = d.experts / d.groups;
-        const uint32_t magic = ((1u << 20) + static_cast<uint32_t>(size) - 1) / static_cast<uint32_t>(size);  // e / size, e and size <= 1024
-        Key mine = none;  // lane g: group g's score
-        for (int g = 0; g < d.groups; ++g) {
-            Key a1 = none, a2 = none;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const uint32_t e = static_cast<uint32_t>(i * 32 + lane);
-                Key k = none;
-                if (static_cast<int>((e * magic) >> 20) == g && key[i] != none) k = d.bias != nullptr ? key[i] : key_of(s[i]);
-                if (k > a1) { a2 = a1; a1 = k; }
-                else if (k > a2) a2 = k;
-            }
-            const Key m1 = warp_max(a1);
-            const int owner = __ffs(__ballot_sync(kFull, a1 == m1)) - 1;
-            const Key m2 = warp_max(lane == owner ? a2 : a1);
-            Key total = none;
-            if (m1 != none) total = key_of(value_of(m1) + (m2 != none ? value_of(m2) : R(0)));
-            if (lane == g) mine = total;
-        }
-        int better = 0;
-        for (int g = 0; g < d.groups; ++g) {
-            const Key other = __shfl_sync(kFull, mine, g);
-            better += other > mine || (other == mine && g < lane) ? 1 : 0;
-        }
-        const bool kept = lane < d.groups && better < d.top_groups;
-        if constexpr (F32) {
-            const Key worst = ~warp_max(kept ? ~mine : Key(0));
-            const Key best = warp_max(!kept && lane < d.groups ? mine : Key(0));
-            if (best > none && !far(value_of(worst), value_of(best))) close = true;
-        }
-        const uint32_t keep = __ballot_sync(kFull, kept);
+    if (d.bias != nullptr || grouped) {
+        R s[VPL];
+        scores<R, VPL>(l, d.sigmoid != 0, top, s);
+        Key ck[VPL];  // by c, which is what groups compare
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const uint32_t g = (static_cast<uint32_t>(i * 32 + lane) * magic) >> 20;
-            if (g >= 32 || !((keep >> g) & 1u)) key[i] = none;
+            const int e = i * 32 + lane;
+            R c = s[i];
+            if (d.bias != nullptr) c += e < d.experts ? R(d.bias[e]) : R(0);
+            ck[i] = l[i] == -INFINITY || !(c > R(-INFINITY)) ? none : key_of(c);
+            key[i] = d.bias != nullptr ? ck[i] : key_of(R(l[i]));
         }
+        if (grouped) {
+            const int size = d.experts / d.groups;
+            const uint32_t magic = ((1u << 20) + static_cast<uint32_t>(size) - 1) / static_cast<uint32_t>(size);  // e / size, e and size <= 1024
+            Key mine = none;  // lane g: group g's score
+            auto total = [&](Key m1, Key m2) {
+                return m1 == none ? none : key_of(value_of(m1) + (m2 != none ? value_of(m2) : R(0)));
+            };
+            if (size % 32 == 0) {  // a group is whole registers
+                const int per = size / 32;
+                Key a1 = none, a2 = none;
+                int left = per, g = 0;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) {
+                    if (ck[i] > a1) { a2 = a1; a1 = ck[i]; }
+                    else if (ck[i] > a2) a2 = ck[i];
+                    if (--left == 0) {
+                        Key m1, m2;
+                        warp_top2(a1, a2, lane, m1, m2);
+                        if (lane == g) mine = total(m1, m2);
+                        ++g;
+                        left = per;
+                        a1 = a2 = none;
+                    }
+                }
+            } else {
+                for (int g = 0; g < d.groups; ++g) {
+                    Key a1 = none, a2 = none;
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) {
+                        const Key k = static_cast<int>((static_cast<uint32_t>(i * 32 + lane) * magic) >> 20) == g ? ck[i] : none;
+                        if (k > a1) { a2 = a1; a1 = k; }
+                        else if (k > a2) a2 = k;
+                    }
+                    Key m1, m2;
+                    warp_top2(a1, a2, lane, m1, m2);
+                    if (lane == g) mine = total(m1, m2);
+                }
+            }
+            int better = 0;
+            for (int g = 0; g < d.groups; ++g) {
+                const Key other = __shfl_sync(kFull, mine, g);
+                better += other > mine || (other == mine && g < lane) ? 1 : 0;
+            }
+            const bool kept = lane < d.groups && better < d.top_groups;
+            if constexpr (F32) {
+                const Key worst = ~warp_max(kept ? ~mine : Key(0));
+                const Key best = warp_max(!kept && lane < d.groups ? mine : Key(0));
+                if (best > none && !far(value_of(worst), value_of(best))) close = true;
+            }
+            const uint32_t keep = __ballot_sync(kFull, kept);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const uint32_t g = (static_cast<uint32_t>(i * 32 + lane) * magic) >> 20;
+                if (g >= 32 || !((keep >> g) & 1u) || ck[i] == none) key[i] = none;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) key[i] = key_of(R(l[i]));
     }
     id = -1;
-    score = R(0);
     Key last = none;
+    Key best = none;  // this lane's best and its register
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+        if (key[i] > best) { best = key[i]; at = i; }
     for (int j = 0; j <= d.top_k; ++j) {  // one more than chosen, for the distance to the first that is not
         if (j == d.top_k && !(F32 && d.bias != nullptr)) break;
-        Key best = none;
-        int at = 0;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (key[i] > best) { best = key[i]; at = i; }
-        const Key top = warp_max(best);
-        if (top == none) break;
+        const Key m = warp_max(best);
+        if (m == none) break;
         if constexpr (F32) {
-            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(top))) close = true;
+            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(m))) close = true;
         }
         if (j == d.top_k) break;
-        last = top;
-        const uint32_t e = __reduce_min_sync(kFull, best == top ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
-        const int owner = static_cast<int>(e & 31u);
-        R v = R(0);
+        last = m;
+        const uint32_t holders = __ballot_sync(kFull, best == m);
+        uint32_t e;
+        if ((holders & (holders - 1)) == 0) {
+            const int owner = __ffs(holders) - 1;
+            e = static_cast<uint32_t>(__shfl_sync(kFull, at, owner) * 32 + owner);
+        } else {  // a tie: the lowest expert
+            e = __reduce_min_sync(kFull, best == m ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
+        }
+        if (lane == j) id = static_cast<int>(e);
+        if (lane == static_cast<int>(e & 31u)) {
+            best = none;
+            const int gone = at;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (lane == owner && i == static_cast<int>(e >> 5)) { v = s[i]; key[i] = none; }
-        v = __shfl_sync(kFull, v, owner);
-        if (lane == j) { id = static_cast<int>(e); score = v; }
+            for (int i = 0; i < VPL; ++i) {
+                if (i == gone) key[i] = none;
+                if (key[i] > best) { best = key[i]; at = i; }
+            }
+        }
     }
     return !close;
+}
+
+template <int VPL>
+__device__ __noinline__ int choose_exactly(const RouteDesc &d, const float (&l)[VPL], float top, int lane) {
+    int id;
+    choose<double, VPL>(d, l, top, lane, id);
+    return id;
 }
 
 // Chooses and writes one token's ids and weights; returns lane j's id.
@@ -195,18 +246,40 @@ __device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, 
     int id = -1;
     float w = 0.0f;
     if (t < live) {
+        const T *row = static_cast<const T *>(d.logits) + static_cast<long long>(t) * d.ld;
         float l[VPL];
-        load_row<T, VPL>(static_cast<const T *>(d.logits) + static_cast<long long>(t) * d.ld, d.experts, lane, l);
-        float s;
-        if (!choose<float, VPL>(d, l, lane, id, s)) {
-            double s64;
-            choose<double, VPL>(d, l, lane, id, s64);
-            s = static_cast<float>(s64);
+        load_row<T, VPL>(row, d.experts, lane, l);
+        const float top = d.sigmoid ? 0.0f : row_top(l);
+        if (!choose<float, VPL>(d, l, top, lane, id)) {
+            float again[VPL];  // a copy of its own: l stays in registers
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) again[i] = l[i];
+            id = choose_exactly<VPL>(d, again, top, lane);
         }
-        w = s;
+        // The chosen ones' scores, one a lane.
+        const float x = id >= 0 ? fminf(to_f32(row[id]), kTop) : -INFINITY;
+        if (d.sigmoid) {
+            w = 1.0f / (1.0f + expf(-x));
+        } else {
+            w = id >= 0 ? expf(x - top) : 0.0f;
+            if (!d.renorm) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) sum += l[i] == -INFINITY ? 0.0f : expf(l[i] - top);
+                sum = warp_sum(sum);
+                w = sum > 0.0f ? w / sum : 0.0f;
+            }
+        }
         if (d.renorm) {
             const float sum = warp_sum(w);
-            w = sum > 0.0f ? w / sum : 0.0f;
+            if (sum >= 1e-30f) {
+                w = w / sum;
+            } else {  // all far below f32's range, or none: as the definition in 64 bits
+                double v = 0.0;
+                if (id >= 0) v = d.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - static_cast<double>(top));
+                const double all = warp_sum(v);
+                w = all > 0.0 ? static_cast<float>(v / all) : 0.0f;
+            }
         }
         w *= d.scale;
     }
@@ -296,7 +369,7 @@ constexpr int kSmallSlots = 1024;
 
 // All in one block: few slots.
 template <typename T, int VPL>
-__global__ void __launch_bounds__(kThreads) k_route_small(const RouteDesc d) {
+__global__ void __launch_bounds__(kThreads) k_route_small(const __grid_constant__ RouteDesc d) {
     extern __shared__ int sm[];
     __shared__ int ids[kSmallSlots];
     grid_dep_wait();
@@ -323,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) k_route_small(const RouteDesc d) {
 
 // Many slots, first kernel: the choice, and the block's count of every expert.
 template <typename T, int VPL>
-__global__ void __launch_bounds__(kThreads) k_route_choose(const RouteDesc d, int per_block) {
+__global__ void __launch_bounds__(kChooseThreads) k_route_choose(const __grid_constant__ RouteDesc d, int per_block) {
     extern __shared__ int sm[];
     grid_dep_wait();
     grid_dep_launch();
@@ -331,23 +404,23 @@ __global__ void __launch_bounds__(kThreads) k_route_choose(const RouteDesc d, in
     const int live = d.token_count != nullptr ? *d.token_count : d.tokens;
     const bool plan = d.offsets != nullptr;
     if (plan) {
-        for (int e = threadIdx.x; e < d.experts; e += kThreads) sm[e] = 0;
+        for (int e = threadIdx.x; e < d.experts; e += kChooseThreads) sm[e] = 0;
         __syncthreads();
     }
     const long long lo = static_cast<long long>(blockIdx.x) * per_block;
     const int hi = static_cast<int>(min(lo + per_block, static_cast<long long>(d.tokens)));
-    for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += kWarps) {
+    for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += kChooseThreads / 32) {
         const int id = route_token<T, VPL>(d, t, live, lane);
         if (plan && id >= 0) atomicAdd(&sm[id], 1);
     }
     if (plan) {
         __syncthreads();
-        for (int e = threadIdx.x; e < d.experts; e += kThreads) d.hist[static_cast<long long>(blockIdx.x) * d.experts + e] = sm[e];
+        for (int e = threadIdx.x; e < d.experts; e += kChooseThreads) d.hist[static_cast<long long>(blockIdx.x) * d.experts + e] = sm[e];
     }
 }
 
 // Second kernel: every block sums the counts (all, and of the blocks before it), then ranks its slots.
-__global__ void __launch_bounds__(kThreads) k_route_plan(const RouteDesc d, int per_block) {
+__global__ void __launch_bounds__(kThreads) k_route_plan(const __grid_constant__ RouteDesc d, int per_block) {
     extern __shared__ int sm[];
     grid_dep_wait();
     grid_dep_launch();
@@ -398,7 +471,7 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
         return e;
     }
     const int per = (d.tokens + blocks - 1) / blocks;
-    cudaError_t e = launch_pdl(k_route_choose<T, VPL>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
+    cudaError_t e = launch_pdl(k_route_choose<T, VPL>, dim3(static_cast<unsigned>(blocks)), dim3(kChooseThreads),
                                static_cast<size_t>(d.experts) * sizeof(int), ctx.stream, 1, d, per);
     ctx.launches++;
     if (e != cudaSuccess || d.offsets == nullptr) return e;
@@ -411,14 +484,14 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
 //   softmax, renormalised: a softmax over the chosen experts alone
 //   otherwise dl = J^T ds, with ds_j = scale * (g_j - sum g w) / S or scale * g_j
 template <typename T, typename TD, int VPL>
-__global__ void __launch_bounds__(256) k_route_backward(const RouteBwdDesc d) {
+__global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ RouteBwdDesc d) {
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
     for (long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < d.tokens; t += static_cast<long long>(gridDim.x) * 8) {
         float l[VPL], s[VPL];
         load_row<T, VPL>(static_cast<const T *>(d.logits) + t * d.ld, d.experts, lane, l);
-        scores<float, VPL>(l, d.sigmoid != 0, s);
+        scores<float, VPL>(l, d.sigmoid != 0, d.sigmoid ? 0.0f : row_top(l), s);
         int id = -1;
         float g = 0.0f;
         if (lane < d.top_k) {
