@@ -53,8 +53,11 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     const uint32_t lo = __reduce_max_sync(kFull, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+// Fast forms for the choice, whose f32 errors it allows for, and accurate ones.
+template <bool FAST> __device__ __forceinline__ float exp_of(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST> __device__ __forceinline__ double exp_of(double x) { return exp(x); }
+template <bool FAST> __device__ __forceinline__ float inverse(float x) { return FAST ? __fdividef(1.0f, x) : 1.0f / x; }
+template <bool FAST> __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
 template <typename R>
 __device__ __forceinline__ R warp_sum(R v) {
 #pragma unroll
@@ -84,17 +87,17 @@ __device__ __forceinline__ float row_top(const float (&l)[VPL]) {
     return value_of(warp_max(key_of(top)));
 }
 // Scores of all experts (masked ones: 0). top: softmax's largest logit.
-template <typename R, int VPL>
+template <bool FAST, typename R, int VPL>
 __device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, float top, R (&s)[VPL]) {
     if (sigmoid) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) s[i] = R(1) / (R(1) + exp_of(-R(l[i])));  // -inf: 1 / inf = 0
+        for (int i = 0; i < VPL; ++i) s[i] = l[i] == -INFINITY ? R(0) : inverse<FAST>(R(1) + exp_of<FAST>(-R(fmaxf(l[i], FAST ? -80.0f : l[i]))));
         return;
     }
     R sum = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-        s[i] = l[i] == -INFINITY ? R(0) : exp_of(R(l[i]) - R(top));
+        s[i] = l[i] == -INFINITY ? R(0) : exp_of<FAST>(R(l[i]) - R(top));
         sum += s[i];
     }
     sum = warp_sum(sum);
@@ -111,21 +114,80 @@ __device__ __forceinline__ void warp_top2(Key a1, Key a2, int lane, Key &m1, Key
     m2 = warp_max(lane == owner ? a2 : a1);
 }
 
+// The top_k largest of the f32 keys, sorted: at least top_k keys reach the top_k-th largest of the lanes' maxima, and
+// usually only a few more do. Those are packed into `buf` (32 entries), ranked against each other and handed to the
+// lanes in order. False if they are more than 32 (many equal keys): the caller takes them one by one.
+// This costs about 220 instructions a token at 256 experts and top_k 8, taking the maximum top_k times 540.
+template <int VPL>
+__device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t (&key)[VPL], int lane, uint2 *buf, int &id, bool &close) {
+    const uint32_t none = key_of(-INFINITY);
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) m = max(m, key[i]);
+    m = max(m, none);
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {  // bitonic, largest in lane 0
+#pragma unroll
+        for (int s = size / 2; s > 0; s /= 2) {
+            const uint32_t o = __shfl_xor_sync(kFull, m, s);
+            const bool up = ((lane & size) == 0) == ((lane & s) == 0);  // this lane keeps the larger
+            m = up ? max(m, o) : min(m, o);
+        }
+    }
+    const uint32_t least = max(__shfl_sync(kFull, m, d.top_k - 1), none + 1);
+    int count = 0;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const bool in = key[i] >= least;
+        const uint32_t who = __ballot_sync(kFull, in);
+        const int at = count + __popc(who & ((1u << lane) - 1u));
+        if (in && at < 32) buf[at] = make_uint2(key[i], static_cast<uint32_t>(i * 32 + lane));
+        count += __popc(who);
+    }
+    if (count > 32) return false;
+    __syncwarp();
+    const uint2 own = lane < count ? buf[lane] : make_uint2(0u, ~0u);
+    int rank = 0;
+    for (int x = 0; x < count; ++x) {
+        const uint2 other = buf[x];
+        rank += other.x > own.x || (other.x == own.x && other.y < own.y) ? 1 : 0;
+    }
+    __syncwarp();
+    if (lane < count) buf[rank] = own;
+    __syncwarp();
+    const uint2 mine = lane < count ? buf[lane] : make_uint2(none, 0u);
+    if (lane < d.top_k && lane < count) id = static_cast<int>(mine.y);
+    if (d.bias != nullptr) {  // the distances between neighbours, down to the first that is not chosen
+        uint32_t rest = none;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) rest = max(rest, key[i] < least ? key[i] : none);
+        rest = warp_max(rest);
+        uint32_t next = __shfl_down_sync(kFull, mine.x, 1);
+        if (lane + 1 >= count) next = rest;
+        const float x = value_of(mine.x), y = value_of(next);
+        const bool near = lane < d.top_k && lane < count && next > none && fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x);
+        close = __any_sync(kFull, near) || close;
+    }
+    return true;
+}
+
 // Chooses a token's experts: lane j < top_k gets the j-th id, or -1. Returns false if f32 values that decide something
 // are too close to call.
 template <typename R, int VPL>
-__device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL], float top, int lane, int &id) {
+__device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL], float top, int lane, uint2 *buf, int &id) {
     using Key = decltype(key_of(R(0)));
     constexpr bool F32 = std::is_same<R, float>::value;
     const Key none = key_of(R(-INFINITY));
     const bool grouped = d.groups > 1 && d.top_groups < d.groups;
     Key key[VPL];
     bool close = false;
-    // f32 error of a score, at most 1, and of its sum with the bias
+    // f32 errors of a score (at most 1; the fast exponential and quotient are off by (2 + 1.2 |x|) and 2 steps of 2^-23,
+    // and what |x| adds the score's own slope takes away) and of its sum with the bias, a few times over
     auto far = [](float x, float y) { return !(fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x)); };
     if (d.bias != nullptr || grouped) {
         R s[VPL];
-        scores<R, VPL>(l, d.sigmoid != 0, top, s);
+        scores<F32, R, VPL>(l, d.sigmoid != 0, top, s);
         Key ck[VPL];  // by c, which is what groups compare
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
@@ -196,6 +258,9 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
         for (int i = 0; i < VPL; ++i) key[i] = key_of(R(l[i]));
     }
     id = -1;
+    if constexpr (F32) {
+        if (choose_sorted<VPL>(d, key, lane, buf, id, close)) return !close;
+    }
     Key last = none;
     Key best = none;  // this lane's best and its register
     int at = 0;
@@ -236,13 +301,13 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
 template <int VPL>
 __device__ __noinline__ int choose_exactly(const RouteDesc &d, const float (&l)[VPL], float top, int lane) {
     int id;
-    choose<double, VPL>(d, l, top, lane, id);
+    choose<double, VPL>(d, l, top, lane, nullptr, id);
     return id;
 }
 
 // Chooses and writes one token's ids and weights; returns lane j's id.
 template <typename T, int VPL>
-__device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, int lane) {
+__device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, int lane, uint2 *buf) {
     int id = -1;
     float w = 0.0f;
     if (t < live) {
@@ -250,7 +315,7 @@ __device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, 
         float l[VPL];
         load_row<T, VPL>(row, d.experts, lane, l);
         const float top = d.sigmoid ? 0.0f : row_top(l);
-        if (!choose<float, VPL>(d, l, top, lane, id)) {
+        if (!choose<float, VPL>(d, l, top, lane, buf, id)) {
             float again[VPL];  // a copy of its own: l stays in registers
 #pragma unroll
             for (int i = 0; i < VPL; ++i) again[i] = l[i];
@@ -372,12 +437,13 @@ template <typename T, int VPL>
 __global__ void __launch_bounds__(kThreads) k_route_small(const __grid_constant__ RouteDesc d) {
     extern __shared__ int sm[];
     __shared__ int ids[kSmallSlots];
+    __shared__ uint2 buf[kWarps * 32];
     grid_dep_wait();
     grid_dep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int live = d.token_count != nullptr ? *d.token_count : d.tokens;
     for (int t = warp; t < d.tokens; t += kWarps) {
-        const int id = route_token<T, VPL>(d, t, live, lane);
+        const int id = route_token<T, VPL>(d, t, live, lane, buf + warp * 32);
         if (lane < d.top_k) ids[t * d.top_k + lane] = id;
     }
     if (d.offsets == nullptr) return;
@@ -398,6 +464,7 @@ __global__ void __launch_bounds__(kThreads) k_route_small(const __grid_constant_
 template <typename T, int VPL>
 __global__ void __launch_bounds__(kChooseThreads) k_route_choose(const __grid_constant__ RouteDesc d, int per_block) {
     extern __shared__ int sm[];
+    __shared__ uint2 buf[kChooseThreads];
     grid_dep_wait();
     grid_dep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -410,7 +477,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_route_choose(const __grid_co
     const long long lo = static_cast<long long>(blockIdx.x) * per_block;
     const int hi = static_cast<int>(min(lo + per_block, static_cast<long long>(d.tokens)));
     for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += kChooseThreads / 32) {
-        const int id = route_token<T, VPL>(d, t, live, lane);
+        const int id = route_token<T, VPL>(d, t, live, lane, buf + warp * 32);
         if (plan && id >= 0) atomicAdd(&sm[id], 1);
     }
     if (plan) {
@@ -432,8 +499,11 @@ __global__ void __launch_bounds__(kThreads) k_route_plan(const __grid_constant__
     for (int i = threadIdx.x; i < experts * parts; i += kThreads) {
         const int e = i % experts, part = i / experts;
         int all = 0, mine = 0;
+        // Each block begins at its own row, so that they do not all read the same lines at once.
 #pragma unroll 8
-        for (int b = part; b < blocks; b += parts) {
+        for (int x = part; x < blocks; x += parts) {
+            int b = x + static_cast<int>(blockIdx.x);
+            if (b >= blocks) b -= blocks;
             const int n = d.hist[static_cast<long long>(b) * experts + e];
             all += n;
             if (b < static_cast<int>(blockIdx.x)) mine += n;
@@ -491,7 +561,7 @@ __global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ 
     for (long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < d.tokens; t += static_cast<long long>(gridDim.x) * 8) {
         float l[VPL], s[VPL];
         load_row<T, VPL>(static_cast<const T *>(d.logits) + t * d.ld, d.experts, lane, l);
-        scores<float, VPL>(l, d.sigmoid != 0, d.sigmoid ? 0.0f : row_top(l), s);
+        scores<false, float, VPL>(l, d.sigmoid != 0, d.sigmoid ? 0.0f : row_top(l), s);
         int id = -1;
         float g = 0.0f;
         if (lane < d.top_k) {
@@ -549,7 +619,8 @@ static cudaError_t with_vpl(int experts, F f) {
 }  // namespace route
 
 int route_blocks(int tokens, int top_k) {
-    if (static_cast<long long>(tokens) * top_k <= route::kSmallSlots) return 0;
+    // One block chooses 16 tokens at a time; past 64 the second launch costs less than the wait.
+    if (tokens <= 64 && static_cast<long long>(tokens) * top_k <= route::kSmallSlots) return 0;
     const int by_tokens = (tokens + route::kWarps - 1) / route::kWarps;
     return by_tokens < 148 ? by_tokens : 148;
 }
