@@ -29,6 +29,7 @@ namespace route {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kPlanThreads = 1024;
 constexpr int kChooseThreads = 1024;  // of the kernel that only chooses: 32 warps hide the reductions' latency
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -114,17 +115,25 @@ __device__ __forceinline__ void warp_top2(Key a1, Key a2, int lane, Key &m1, Key
     m2 = warp_max(lane == owner ? a2 : a1);
 }
 
-// The top_k largest of the f32 keys, sorted: at least top_k keys reach the top_k-th largest of the lanes' maxima, and
-// usually only a few more do. Those are packed into `buf` (32 entries), ranked against each other and handed to the
-// lanes in order. False if they are more than 32 (many equal keys): the caller takes them one by one.
-// This costs about 220 instructions a token at 256 experts and top_k 8, taking the maximum top_k times 540.
+// How far an f32 value of c may be from its exact value. Sigmoid: the fast exponential's (2 + 1.2 |x|) steps of 2^-23
+// times the slope s (1 - s), at most 7e-8; two steps for the quotient and one for 1 + e, 3.1e-7. Softmax: s <= 1 times
+// the sum's relative error, (2 + 1.2 ln 1024) steps of its terms and up to 37 additions, 4.1e-6. Then the sum with the
+// bias, half a step of c.
+__device__ __forceinline__ float doubt(const RouteDesc &d, float c) { return (d.sigmoid ? 5e-7f : 5e-6f) + 1e-7f * fabsf(c); }
+
+// The top_k largest of the f32 keys, in order, to lanes 0 .. top_k - 1. At least top_k keys reach the top_k-th largest of
+// the lanes' maxima, and usually only a few more do. Those (and, with a bias, the ones that may belong to them) are
+// packed into `buf` (32 entries) and ranked against each other. Where neighbours are too close to call, each lane
+// computes its candidate's c again in f64 and they are ranked by that.
+// False if there are more than 32 candidates (many equal keys): the caller takes them one by one.
+// About 220 instructions a token at 256 experts and top_k 8; taking the maximum top_k times costs 540.
 template <int VPL>
-__device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t (&key)[VPL], int lane, uint2 *buf, int &id, bool &close) {
+__device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t (&key)[VPL], const float (&l)[VPL], float top, int lane,
+                                              uint2 *buf, int &id) {
     const uint32_t none = key_of(-INFINITY);
     uint32_t m = key[0];
 #pragma unroll
     for (int i = 1; i < VPL; ++i) m = max(m, key[i]);
-    m = max(m, none);
 #pragma unroll
     for (int size = 2; size <= 32; size *= 2) {  // bitonic, largest in lane 0
 #pragma unroll
@@ -134,7 +143,12 @@ __device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t
             m = up ? max(m, o) : min(m, o);
         }
     }
-    const uint32_t least = max(__shfl_sync(kFull, m, d.top_k - 1), none + 1);
+    uint32_t least = __shfl_sync(kFull, m, d.top_k - 1);
+    if (d.bias != nullptr && least > none) {
+        const float v = value_of(least);
+        least = key_of(v - 2.0f * doubt(d, v));
+    }
+    least = max(least, none + 1);
     int count = 0;
     __syncwarp();
 #pragma unroll
@@ -149,26 +163,52 @@ __device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t
     __syncwarp();
     const uint2 own = lane < count ? buf[lane] : make_uint2(0u, ~0u);
     int rank = 0;
+    bool near = false;
+    const float c = value_of(own.x), reach = 2.0f * doubt(d, c);
     for (int x = 0; x < count; ++x) {
         const uint2 other = buf[x];
         rank += other.x > own.x || (other.x == own.x && other.y < own.y) ? 1 : 0;
+        near |= x != lane && fabsf(value_of(other.x) - c) <= reach;
+    }
+    near = near && lane < count && rank <= d.top_k;
+    if (d.bias != nullptr && __any_sync(kFull, near)) {
+        double total = 0.0;
+        if (!d.sigmoid) {
+#pragma unroll 1
+            for (int q = 0; q < VPL; ++q) {  // one copy of the f64 exponential: the register is picked by comparison
+                float v = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (i == q) v = l[i];
+                total += v == -INFINITY ? 0.0 : exp(static_cast<double>(v) - static_cast<double>(top));
+            }
+            total = warp_sum(total);
+        }
+        float x_own = 0.0f;  // the candidate's logit, from the lane that holds it
+#pragma unroll
+        for (int q = 0; q < VPL; ++q) {
+            const float v = __shfl_sync(kFull, l[q], own.y & 31u);
+            if (q == static_cast<int>(own.y >> 5)) x_own = v;
+        }
+        double exact = 0.0;
+        uint64_t k64 = 0;
+        if (lane < count) {
+            const int e = static_cast<int>(own.y);
+            const double v = x_own;
+            exact = (d.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - static_cast<double>(top)) / total) + static_cast<double>(d.bias[e]);
+            k64 = key_of(exact);
+        }
+        rank = 0;
+        for (int x = 0; x < count; ++x) {
+            const uint64_t other = __shfl_sync(kFull, k64, x);
+            const uint32_t e = __shfl_sync(kFull, own.y, x);
+            rank += other > k64 || (other == k64 && e < own.y) ? 1 : 0;
+        }
     }
     __syncwarp();
     if (lane < count) buf[rank] = own;
     __syncwarp();
-    const uint2 mine = lane < count ? buf[lane] : make_uint2(none, 0u);
-    if (lane < d.top_k && lane < count) id = static_cast<int>(mine.y);
-    if (d.bias != nullptr) {  // the distances between neighbours, down to the first that is not chosen
-        uint32_t rest = none;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) rest = max(rest, key[i] < least ? key[i] : none);
-        rest = warp_max(rest);
-        uint32_t next = __shfl_down_sync(kFull, mine.x, 1);
-        if (lane + 1 >= count) next = rest;
-        const float x = value_of(mine.x), y = value_of(next);
-        const bool near = lane < d.top_k && lane < count && next > none && fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x);
-        close = __any_sync(kFull, near) || close;
-    }
+    if (lane < d.top_k && lane < count) id = static_cast<int>(buf[lane].y);
     return true;
 }
 
@@ -182,9 +222,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
     const bool grouped = d.groups > 1 && d.top_groups < d.groups;
     Key key[VPL];
     bool close = false;
-    // f32 errors of a score (at most 1; the fast exponential and quotient are off by (2 + 1.2 |x|) and 2 steps of 2^-23,
-    // and what |x| adds the score's own slope takes away) and of its sum with the bias, a few times over
-    auto far = [](float x, float y) { return !(fabsf(x - y) <= 8e-6f + 5e-7f * fabsf(x)); };
+    auto far = [&](float x, float y, float terms) { return !(fabsf(x - y) <= 2.0f * terms * doubt(d, x)); };
     if (d.bias != nullptr || grouped) {
         R s[VPL];
         scores<F32, R, VPL>(l, d.sigmoid != 0, top, s);
@@ -244,7 +282,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             if constexpr (F32) {
                 const Key worst = ~warp_max(kept ? ~mine : Key(0));
                 const Key best = warp_max(!kept && lane < d.groups ? mine : Key(0));
-                if (best > none && !far(value_of(worst), value_of(best))) close = true;
+                if (best > none && !far(value_of(worst), value_of(best), 2.0f)) close = true;
             }
             const uint32_t keep = __ballot_sync(kFull, kept);
 #pragma unroll
@@ -259,7 +297,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
     }
     id = -1;
     if constexpr (F32) {
-        if (choose_sorted<VPL>(d, key, lane, buf, id, close)) return !close;
+        if (!close && choose_sorted<VPL>(d, key, l, top, lane, buf, id)) return true;
     }
     Key last = none;
     Key best = none;  // this lane's best and its register
@@ -272,7 +310,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
         const Key m = warp_max(best);
         if (m == none) break;
         if constexpr (F32) {
-            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(m))) close = true;
+            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(m), 1.0f)) close = true;
         }
         if (j == d.top_k) break;
         last = m;
@@ -381,11 +419,13 @@ __device__ void expert_bases(const int *count, int *base, int experts, int align
 
 // Rows of slots [lo, hi) of this block: next[w * experts + e] first counts warp w's slots of expert e, then becomes the
 // row of its next one. `first` gives each expert's first row for this block.
+template <int THREADS>
 __device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, long long hi, int *next, const int *first, int experts) {
+    constexpr int WARPS = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long per = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const long long per = ((hi - lo + WARPS - 1) / WARPS + 31) / 32 * 32;
     const long long a = min(lo + warp * per, hi), b = min(a + per, hi);
-    for (int i = threadIdx.x; i < kWarps * experts; i += kThreads) next[i] = 0;
+    for (int i = threadIdx.x; i < WARPS * experts; i += THREADS) next[i] = 0;
     __syncthreads();
     for (long long i = a; i < b; i += 32) {
         const int e = i + lane < b ? ids[i + lane - lo] : -1;
@@ -394,10 +434,10 @@ __device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, lon
         __syncwarp();
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kThreads) {
+    for (int e = threadIdx.x; e < experts; e += THREADS) {
         int at = first[e];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const int n = next[w * experts + e];
             next[w * experts + e] = at;
             at += n;
@@ -420,13 +460,14 @@ __device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, lon
 }
 
 // Rows that hold no slot: the padding behind an expert's rows, and the rows behind the last expert.
+template <int THREADS>
 __device__ void fill_padding(const RouteDesc &d, const int *count, const int *base, int block, int blocks) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (d.align > 1)
-        for (int e = block * kWarps + warp; e < d.experts; e += blocks * kWarps)
+        for (int e = block * (THREADS / 32) + warp; e < d.experts; e += blocks * (THREADS / 32))
             for (int r = base[e] + count[e] + lane; r < min(base[e + 1], d.rows); r += 32) d.row_slot[r] = -1;
-    for (long long r = base[d.experts] + static_cast<long long>(block) * kThreads + threadIdx.x; r < d.rows;
-         r += static_cast<long long>(blocks) * kThreads)
+    for (long long r = base[d.experts] + static_cast<long long>(block) * THREADS + threadIdx.x; r < d.rows;
+         r += static_cast<long long>(blocks) * THREADS)
         d.row_slot[r] = -1;
 }
 
@@ -456,8 +497,8 @@ __global__ void __launch_bounds__(kThreads) k_route_small(const __grid_constant_
     __syncthreads();
     expert_bases(count, base, d.experts, d.align);
     for (int e = threadIdx.x; e <= d.experts; e += kThreads) d.offsets[e] = base[e];
-    rank_slots(d, ids, 0, slots, next, base, d.experts);
-    fill_padding(d, count, base, 0, 1);
+    rank_slots<kThreads>(d, ids, 0, slots, next, base, d.experts);
+    fill_padding<kThreads>(d, count, base, 0, 1);
 }
 
 // Many slots, first kernel: the choice, and the block's count of every expert.
@@ -487,16 +528,16 @@ __global__ void __launch_bounds__(kChooseThreads) k_route_choose(const __grid_co
 }
 
 // Second kernel: every block sums the counts (all, and of the blocks before it), then ranks its slots.
-__global__ void __launch_bounds__(kThreads) k_route_plan(const __grid_constant__ RouteDesc d, int per_block) {
+__global__ void __launch_bounds__(kPlanThreads) k_route_plan(const __grid_constant__ RouteDesc d, int per_block) {
     extern __shared__ int sm[];
     grid_dep_wait();
     grid_dep_launch();
     const int experts = d.experts;
     int *count = sm, *before = count + experts, *base = before + experts, *next = base + experts + 1;
-    for (int i = threadIdx.x; i < 2 * experts; i += kThreads) sm[i] = 0;
+    for (int i = threadIdx.x; i < 2 * experts; i += kPlanThreads) sm[i] = 0;
     __syncthreads();
-    const int parts = max(1, kThreads / experts), blocks = gridDim.x;
-    for (int i = threadIdx.x; i < experts * parts; i += kThreads) {
+    const int parts = max(1, kPlanThreads / experts), blocks = gridDim.x;
+    for (int i = threadIdx.x; i < experts * parts; i += kPlanThreads) {
         const int e = i % experts, part = i / experts;
         int all = 0, mine = 0;
         // Each block begins at its own row, so that they do not all read the same lines at once.
@@ -514,25 +555,24 @@ __global__ void __launch_bounds__(kThreads) k_route_plan(const __grid_constant__
     __syncthreads();
     expert_bases(count, base, experts, d.align);
     if (blockIdx.x == 0)
-        for (int e = threadIdx.x; e <= experts; e += kThreads) d.offsets[e] = base[e];
-    for (int e = threadIdx.x; e < experts; e += kThreads) before[e] += base[e];
+        for (int e = threadIdx.x; e <= experts; e += kPlanThreads) d.offsets[e] = base[e];
+    for (int e = threadIdx.x; e < experts; e += kPlanThreads) before[e] += base[e];
     __syncthreads();
     const long long slots = static_cast<long long>(d.tokens) * d.top_k;
     const long long lo = min(static_cast<long long>(blockIdx.x) * per_block * d.top_k, slots);
     const long long hi = min(lo + static_cast<long long>(per_block) * d.top_k, slots);
-    rank_slots(d, d.ids + lo, lo, hi, next, before, experts);
-    fill_padding(d, count, base, blockIdx.x, blocks);
+    rank_slots<kPlanThreads>(d, d.ids + lo, lo, hi, next, before, experts);
+    fill_padding<kPlanThreads>(d, count, base, blockIdx.x, blocks);
 }
 
 template <typename T, int VPL>
 static cudaError_t launch(Context &ctx, const RouteDesc &d) {
     const int blocks = route_blocks(d.tokens, d.top_k);
-    const size_t plan_ints = static_cast<size_t>(d.experts) * (kWarps + 3) + 1;
-    const size_t smem = plan_ints * sizeof(int);
-    if (smem > 40 * 1024) {  // with the static 4 KiB still within the 48 KiB that need no opt-in
-        cudaError_t e = cudaFuncSetAttribute(k_route_small<T, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(k_route_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // count, bases and every warp's counters; the plan kernel's own counts besides
+    const size_t smem = (static_cast<size_t>(d.experts) * (blocks == 0 ? kWarps + 2 : kPlanThreads / 32 + 3) + 1) * sizeof(int);
+    if (smem > 32 * 1024) {  // with the static arrays past the 48 KiB that need no opt-in
+        const cudaError_t e = blocks == 0 ? cudaFuncSetAttribute(k_route_small<T, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))
+                                          : cudaFuncSetAttribute(k_route_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;
     }
     if (blocks == 0) {
@@ -545,7 +585,7 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
                                static_cast<size_t>(d.experts) * sizeof(int), ctx.stream, 1, d, per);
     ctx.launches++;
     if (e != cudaSuccess || d.offsets == nullptr) return e;
-    e = launch_pdl(k_route_plan, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, ctx.stream, 1, d, per);
+    e = launch_pdl(k_route_plan, dim3(static_cast<unsigned>(blocks)), dim3(kPlanThreads), smem, ctx.stream, 1, d, per);
     ctx.launches++;
     return e;
 }
