@@ -319,6 +319,8 @@ gs_status gs_moe_route(gs_handle h, const gs_route_desc *q) {
             d.sigmoid = q->score == GS_ROUTE_SIGMOID;
             d.groups = q->groups;
             d.top_groups = q->top_groups;
+            d.group_size = q->experts / q->groups;
+            d.group_magic = ((1u << 20) + static_cast<uint32_t>(d.group_size) - 1) / static_cast<uint32_t>(d.group_size);
             d.renorm = q->renormalize != 0;
             d.scale = q->scale;
             d.token_count = q->token_count;

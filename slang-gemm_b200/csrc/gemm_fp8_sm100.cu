@@ -271,9 +271,9 @@ __device__ __forceinline__ bool mbar_wait2(uint64_t *b1, uint32_t parity1, uint3
     return (r1 || mbar_wait(b1, parity1, err, site1, limit)) && (r2 || mbar_wait(b2, parity2, err, site2, limit));
 }
 
-// 4-byte asynchronous copy global -> shared; zeros where `in` is false.
-__device__ __forceinline__ void cp_async_f32(uint32_t dst, const float *src, bool in) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+// 4-byte asynchronous copy global -> shared.
+__device__ __forceinline__ void cp_async_f32(uint32_t dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // Arrives on the barrier when this thread's earlier cp.async have completed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
@@ -530,38 +530,30 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         uint32_t sp = 0;
         bool ok = true;
         for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
-            const float *pp = args.p.scale + it.g * args.p.s_g, *pq = args.q.scale + it.g * args.q.s_g;
+            // This lane's first scale of either side (a scale per vector has its non-K index contiguous), and which of its
+            // copies lie inside. What is not copied scales rows and columns that are not stored.
+            constexpr int NP = P_VEC ? BM / 32 : 1, NQ = Q_VEC ? BN / 32 : 1;
+            const int pi = P_VEC ? it.p0 + lane : it.p0 / 128, qi = Q_VEC ? it.q0 + lane : it.q0 / 128 + lane;
+            const float *pp = args.p.scale + it.g * args.p.s_g + pi * args.p.s_i + it.kb0 * args.p.s_k;
+            const float *pq = args.q.scale + it.g * args.q.s_g + qi * args.q.s_i + it.kb0 * args.q.s_k;
+            const int np = P_VEC ? (it.p_end - pi + 31) / 32 : (lane == 0 && it.p0 < it.p_end ? 1 : 0);
+            const int nq = Q_VEC ? (it.q_end - qi + 31) / 32 : (lane < (BN + 127) / 128 && it.q0 + lane * 128 < it.q_end ? 1 : 0);
             for (int kb = 0; kb < it.nkb; ++kb) {
                 // one answer for the warp: its lanes arrive together
                 if (!__all_sync(0xffffffffu, mbar_wait(&sempty[ss], sp ^ 1u, args.err, 6, args.spin_limit))) {
                     ok = false;
                     break;
                 }
-                const uint32_t dst = smem_u32(scales + ss * C_::SC_FLOATS);
-                const long long k = it.kb0 + kb;
-                if constexpr (Q_VEC) {
+                const uint32_t dst = smem_u32(scales + ss * C_::SC_FLOATS) + lane * 4;
 #pragma unroll
-                    for (int i = 0; i < BN / 32; ++i) {
-                        const int c = it.q0 + i * 32 + lane;
-                        const bool in = c < it.q_end;
-                        cp_async_f32(dst + (i * 32 + lane) * 4, in ? pq + c * args.q.s_i + k * args.q.s_k : pq, in);
-                    }
-                } else if (lane < (BN + 127) / 128) {
-                    const bool in = it.q0 + lane * 128 < it.q_end;
-                    cp_async_f32(dst + lane * 4, in ? pq + (it.q0 / 128 + lane) * args.q.s_i + k * args.q.s_k : pq, in);
-                }
-                if constexpr (P_VEC) {
+                for (int i = 0; i < NQ; ++i)
+                    if (i < nq) cp_async_f32(dst + i * 128, pq + i * 32);
 #pragma unroll
-                    for (int i = 0; i < BM / 32; ++i) {
-                        const int r = it.p0 + i * 32 + lane;
-                        const bool in = r < it.p_end;
-                        cp_async_f32(dst + (BN + i * 32 + lane) * 4, in ? pp + r * args.p.s_i + k * args.p.s_k : pp, in);
-                    }
-                } else if (lane == 0) {
-                    const bool in = it.p0 < it.p_end;
-                    cp_async_f32(dst + BN * 4, in ? pp + it.p0 / 128 * args.p.s_i + k * args.p.s_k : pp, in);
-                }
+                for (int i = 0; i < NP; ++i)
+                    if (i < np) cp_async_f32(dst + BN * 4 + i * 128, pp + i * 32);
                 cp_async_arrive(&sfull[ss]);
+                pp += args.p.s_k;
+                pq += args.q.s_k;
                 if (++ss == SC_STAGES) { ss = 0; sp ^= 1u; }
             }
         }

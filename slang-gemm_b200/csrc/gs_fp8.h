@@ -44,6 +44,7 @@ struct RouteDesc {
     const void *logits; int type; long long ld;
     const float *bias;
     int sigmoid, groups, top_groups, renorm;
+    int group_size; uint32_t group_magic;  // expert e's group is e * group_magic >> 20 (e and group_size <= 1024)
     float scale;
     const int32_t *token_count;
     int align;

@@ -30,7 +30,8 @@ namespace route {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPlanThreads = 1024;
-constexpr int kChooseThreads = 1024;  // of the kernel that only chooses: 32 warps hide the reductions' latency
+// Threads of the kernel that only chooses: 32 warps hide the reductions' latency, where their registers allow it.
+constexpr int choose_threads(int vpl) { return vpl >= 16 ? 512 : 1024; }
 constexpr uint32_t kFull = 0xffffffffu;
 
 // Order-preserving keys. -0 and 0 are one value.
@@ -236,43 +237,29 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             key[i] = d.bias != nullptr ? ck[i] : key_of(R(l[i]));
         }
         if (grouped) {
-            const int size = d.experts / d.groups;
-            const uint32_t magic = ((1u << 20) + static_cast<uint32_t>(size) - 1) / static_cast<uint32_t>(size);  // e / size, e and size <= 1024
-            Key mine = none;  // lane g: group g's score
-            auto total = [&](Key m1, Key m2) {
-                return m1 == none ? none : key_of(value_of(m1) + (m2 != none ? value_of(m2) : R(0)));
+            const int size = d.group_size;
+            Key k1 = none, k2 = none;  // lane g: group g's two best
+            auto record = [&](Key a1, Key a2, int g) {
+                Key m1, m2;
+                warp_top2(a1, a2, lane, m1, m2);
+                if (lane == g) { k1 = m1; k2 = m2; }
             };
-            if (size % 32 == 0) {  // a group is whole registers
-                const int per = size / 32;
-                Key a1 = none, a2 = none;
-                int left = per, g = 0;
+            if (size == 32) {  // a group is a register
 #pragma unroll
-                for (int i = 0; i < VPL; ++i) {
-                    if (ck[i] > a1) { a2 = a1; a1 = ck[i]; }
-                    else if (ck[i] > a2) a2 = ck[i];
-                    if (--left == 0) {
-                        Key m1, m2;
-                        warp_top2(a1, a2, lane, m1, m2);
-                        if (lane == g) mine = total(m1, m2);
-                        ++g;
-                        left = per;
-                        a1 = a2 = none;
-                    }
-                }
+                for (int i = 0; i < VPL; ++i) record(ck[i], none, i);
             } else {
                 for (int g = 0; g < d.groups; ++g) {
                     Key a1 = none, a2 = none;
 #pragma unroll
                     for (int i = 0; i < VPL; ++i) {
-                        const Key k = static_cast<int>((static_cast<uint32_t>(i * 32 + lane) * magic) >> 20) == g ? ck[i] : none;
+                        const Key k = static_cast<int>((static_cast<uint32_t>(i * 32 + lane) * d.group_magic) >> 20) == g ? ck[i] : none;
                         if (k > a1) { a2 = a1; a1 = k; }
                         else if (k > a2) a2 = k;
                     }
-                    Key m1, m2;
-                    warp_top2(a1, a2, lane, m1, m2);
-                    if (lane == g) mine = total(m1, m2);
+                    record(a1, a2, g);
                 }
             }
+            const Key mine = k1 == none ? none : key_of(value_of(k1) + (k2 != none ? value_of(k2) : R(0)));
             int better = 0;
             for (int g = 0; g < d.groups; ++g) {
                 const Key other = __shfl_sync(kFull, mine, g);
@@ -287,7 +274,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             const uint32_t keep = __ballot_sync(kFull, kept);
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
-                const uint32_t g = (static_cast<uint32_t>(i * 32 + lane) * magic) >> 20;
+                const uint32_t g = size == 32 ? static_cast<uint32_t>(i) : (static_cast<uint32_t>(i * 32 + lane) * d.group_magic) >> 20;
                 if (g >= 32 || !((keep >> g) & 1u) || ck[i] == none) key[i] = none;
             }
         }
@@ -396,12 +383,15 @@ __device__ __forceinline__ int route_token(const RouteDesc &d, int t, int live, 
 
 // Exclusive sums over the experts of their aligned counts: base[e] = first row of expert e, base[experts] = all rows.
 // Called by the whole block; `count` and `base` in shared memory.
+template <int THREADS>
 __device__ void expert_bases(const int *count, int *base, int experts, int align) {
+    for (int e = threadIdx.x; e < experts; e += THREADS) base[e] = align == 1 ? count[e] : (count[e] + align - 1) / align * align;
+    __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x, per = (experts + 31) / 32;
         const int lo = min(lane * per, experts), hi = min(lo + per, experts);
         int sum = 0;
-        for (int e = lo; e < hi; ++e) sum += (count[e] + align - 1) / align * align;
+        for (int e = lo; e < hi; ++e) sum += base[e];
         int incl = sum;
         for (int s = 1; s < 32; s <<= 1) {
             const int v = __shfl_up_sync(kFull, incl, s);
@@ -409,48 +399,58 @@ __device__ void expert_bases(const int *count, int *base, int experts, int align
         }
         int at = incl - sum;
         for (int e = lo; e < hi; ++e) {
+            const int n = base[e];
             base[e] = at;
-            at += (count[e] + align - 1) / align * align;
+            at += n;
         }
         if (lane == 31) base[experts] = incl;
     }
     __syncthreads();
 }
 
-// Rows of slots [lo, hi) of this block: next[w * experts + e] first counts warp w's slots of expert e, then becomes the
-// row of its next one. `first` gives each expert's first row for this block.
+// Slots [lo, hi) of a block, a run of whole 32s to a warp: this warp's run.
 template <int THREADS>
-__device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, long long hi, int *next, const int *first, int experts) {
+__device__ __forceinline__ void warp_run(long long lo, long long hi, long long &a, long long &b) {
+    const long long per = ((hi - lo + THREADS / 32 - 1) / (THREADS / 32) + 31) / 32 * 32;
+    a = min(lo + (threadIdx.x >> 5) * per, hi);
+    b = min(a + per, hi);
+}
+
+// Rows of slots [lo, hi) of this block: next[w * ld + e] first counts warp w's slots of expert e, then becomes the row of
+// its next one. `first` gives each expert's first row for this block; `ahead` is this thread's id of its warp's first 32.
+template <int THREADS>
+__device__ void rank_slots(const RouteDesc &d, const int *ids, long long lo, long long hi, int *next, const int *first, int experts, int ahead) {
     constexpr int WARPS = THREADS / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long per = ((hi - lo + WARPS - 1) / WARPS + 31) / 32 * 32;
-    const long long a = min(lo + warp * per, hi), b = min(a + per, hi);
-    for (int i = threadIdx.x; i < WARPS * experts; i += THREADS) next[i] = 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ld = experts | 1;  // odd: an expert's counters lie in different banks
+    long long a, b;
+    warp_run<THREADS>(lo, hi, a, b);
+    for (int i = threadIdx.x; i < WARPS * ld; i += THREADS) next[i] = 0;
     __syncthreads();
     for (long long i = a; i < b; i += 32) {
-        const int e = i + lane < b ? ids[i + lane - lo] : -1;
+        const int e = i == a ? ahead : i + lane < b ? ids[i + lane - lo] : -1;
         const uint32_t same = __match_any_sync(kFull, e);
-        if (e >= 0 && lane == __ffs(same) - 1) next[warp * experts + e] += __popc(same);
+        if (e >= 0 && lane == __ffs(same) - 1) next[warp * ld + e] += __popc(same);
         __syncwarp();
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += THREADS) {
-        int at = first[e];
+    for (int e = warp; e < experts; e += WARPS) {  // a warp sums an expert's counters, one a lane
+        const int n = lane < WARPS ? next[lane * ld + e] : 0;
+        int incl = n;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const int n = next[w * experts + e];
-            next[w * experts + e] = at;
-            at += n;
+        for (int s = 1; s < 32; s <<= 1) {
+            const int v = __shfl_up_sync(kFull, incl, s);
+            if (lane >= s) incl += v;
         }
+        if (lane < WARPS) next[lane * ld + e] = first[e] + incl - n;
     }
     __syncthreads();
     for (long long i = a; i < b; i += 32) {
-        const int e = i + lane < b ? ids[i + lane - lo] : -1;
+        const int e = i == a ? ahead : i + lane < b ? ids[i + lane - lo] : -1;
         const uint32_t same = __match_any_sync(kFull, e);
         int row = -1;
-        if (e >= 0) row = next[warp * experts + e] + __popc(same & ((1u << lane) - 1u));
+        if (e >= 0) row = next[warp * ld + e] + __popc(same & ((1u << lane) - 1u));
         __syncwarp();
-        if (e >= 0 && lane == __ffs(same) - 1) next[warp * experts + e] += __popc(same);
+        if (e >= 0 && lane == __ffs(same) - 1) next[warp * ld + e] += __popc(same);
         __syncwarp();
         if (i + lane < b) {
             d.slot_row[i + lane] = row;
@@ -495,35 +495,38 @@ __global__ void __launch_bounds__(kThreads) k_route_small(const __grid_constant_
     for (int i = threadIdx.x; i < slots; i += kThreads)
         if (ids[i] >= 0) atomicAdd(&count[ids[i]], 1);  // whole numbers: any order gives the same sum
     __syncthreads();
-    expert_bases(count, base, d.experts, d.align);
+    expert_bases<kThreads>(count, base, d.experts, d.align);
     for (int e = threadIdx.x; e <= d.experts; e += kThreads) d.offsets[e] = base[e];
-    rank_slots<kThreads>(d, ids, 0, slots, next, base, d.experts);
+    long long a, b;
+    warp_run<kThreads>(0, slots, a, b);
+    rank_slots<kThreads>(d, ids, 0, slots, next, base, d.experts, a + lane < b ? ids[a + lane] : -1);
     fill_padding<kThreads>(d, count, base, 0, 1);
 }
 
 // Many slots, first kernel: the choice, and the block's count of every expert.
 template <typename T, int VPL>
-__global__ void __launch_bounds__(kChooseThreads) k_route_choose(const __grid_constant__ RouteDesc d, int per_block) {
+__global__ void __launch_bounds__(choose_threads(VPL)) k_route_choose(const __grid_constant__ RouteDesc d, int per_block) {
+    constexpr int THREADS = choose_threads(VPL);
     extern __shared__ int sm[];
-    __shared__ uint2 buf[kChooseThreads];
+    __shared__ uint2 buf[THREADS];
     grid_dep_wait();
     grid_dep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int live = d.token_count != nullptr ? *d.token_count : d.tokens;
     const bool plan = d.offsets != nullptr;
     if (plan) {
-        for (int e = threadIdx.x; e < d.experts; e += kChooseThreads) sm[e] = 0;
+        for (int e = threadIdx.x; e < d.experts; e += THREADS) sm[e] = 0;
         __syncthreads();
     }
     const long long lo = static_cast<long long>(blockIdx.x) * per_block;
     const int hi = static_cast<int>(min(lo + per_block, static_cast<long long>(d.tokens)));
-    for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += kChooseThreads / 32) {
+    for (int t = static_cast<int>(min(lo, static_cast<long long>(hi))) + warp; t < hi; t += THREADS / 32) {
         const int id = route_token<T, VPL>(d, t, live, lane, buf + warp * 32);
         if (plan && id >= 0) atomicAdd(&sm[id], 1);
     }
     if (plan) {
         __syncthreads();
-        for (int e = threadIdx.x; e < d.experts; e += kChooseThreads) d.hist[static_cast<long long>(blockIdx.x) * d.experts + e] = sm[e];
+        for (int e = threadIdx.x; e < d.experts; e += THREADS) d.hist[static_cast<long long>(blockIdx.x) * d.experts + e] = sm[e];
     }
 }
 
@@ -534,6 +537,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_route_plan(const __grid_consta
     grid_dep_launch();
     const int experts = d.experts;
     int *count = sm, *before = count + experts, *base = before + experts, *next = base + experts + 1;
+    const long long slots = static_cast<long long>(d.tokens) * d.top_k;
+    const long long lo = min(static_cast<long long>(blockIdx.x) * per_block * d.top_k, slots);
+    const long long hi = min(lo + static_cast<long long>(per_block) * d.top_k, slots);
+    long long a, b;
+    warp_run<kPlanThreads>(lo, hi, a, b);
+    const int ahead = a + static_cast<int>(threadIdx.x & 31) < b ? d.ids[a + (threadIdx.x & 31)] : -1;  // while the counts come in
     for (int i = threadIdx.x; i < 2 * experts; i += kPlanThreads) sm[i] = 0;
     __syncthreads();
     const int parts = max(1, kPlanThreads / experts), blocks = gridDim.x;
@@ -553,15 +562,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_route_plan(const __grid_consta
         atomicAdd(&before[e], mine);
     }
     __syncthreads();
-    expert_bases(count, base, experts, d.align);
+    expert_bases<kPlanThreads>(count, base, experts, d.align);
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e <= experts; e += kPlanThreads) d.offsets[e] = base[e];
     for (int e = threadIdx.x; e < experts; e += kPlanThreads) before[e] += base[e];
     __syncthreads();
-    const long long slots = static_cast<long long>(d.tokens) * d.top_k;
-    const long long lo = min(static_cast<long long>(blockIdx.x) * per_block * d.top_k, slots);
-    const long long hi = min(lo + static_cast<long long>(per_block) * d.top_k, slots);
-    rank_slots<kPlanThreads>(d, d.ids + lo, lo, hi, next, before, experts);
+    rank_slots<kPlanThreads>(d, d.ids + lo, lo, hi, next, before, experts, ahead);
     fill_padding<kPlanThreads>(d, count, base, blockIdx.x, blocks);
 }
 
@@ -569,7 +575,7 @@ template <typename T, int VPL>
 static cudaError_t launch(Context &ctx, const RouteDesc &d) {
     const int blocks = route_blocks(d.tokens, d.top_k);
     // count, bases and every warp's counters; the plan kernel's own counts besides
-    const size_t smem = (static_cast<size_t>(d.experts) * (blocks == 0 ? kWarps + 2 : kPlanThreads / 32 + 3) + 1) * sizeof(int);
+    const size_t smem = (static_cast<size_t>(d.experts | 1) * (blocks == 0 ? kWarps : kPlanThreads / 32) + static_cast<size_t>(d.experts) * (blocks == 0 ? 2 : 3) + 1) * sizeof(int);
     if (smem > 32 * 1024) {  // with the static arrays past the 48 KiB that need no opt-in
         const cudaError_t e = blocks == 0 ? cudaFuncSetAttribute(k_route_small<T, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))
                                           : cudaFuncSetAttribute(k_route_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -581,7 +587,7 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
         return e;
     }
     const int per = (d.tokens + blocks - 1) / blocks;
-    cudaError_t e = launch_pdl(k_route_choose<T, VPL>, dim3(static_cast<unsigned>(blocks)), dim3(kChooseThreads),
+    cudaError_t e = launch_pdl(k_route_choose<T, VPL>, dim3(static_cast<unsigned>(blocks)), dim3(choose_threads(VPL)),
                                static_cast<size_t>(d.experts) * sizeof(int), ctx.stream, 1, d, per);
     ctx.launches++;
     if (e != cudaSuccess || d.offsets == nullptr) return e;
