@@ -107,7 +107,9 @@ Refusal check_gemm(int ragged, int transa, int transb, int m, int n, int k, int 
         return {};
     }
     if (m > kMaxDim || n > kMaxDim || k > kMaxDim) return unsupported("m, n and k are limited to 2^31 - 1025");
-    if (static_cast<long long>(blocks128(m)) * (n / 32 + (groups > 0 ? groups : 1)) > kMaxDim) return unsupported("too many tiles");
+    // tiles of the smallest kind, and one more round of them, are counted in 32 bits
+    const long long across = n / 32 + (ragged_n ? groups : 1);
+    if (across > kMaxDim / blocks128(m) || (groups > 0 && !ragged_n && across * blocks128(m) > kMaxDim / groups)) return unsupported("too many tiles");
     if (!C || !on(C, float_size(ct))) return invalid("C is null or misaligned");
     if (k > 0) {
         if (!A || !B || !sa || !sb) return invalid("null operand or scale");

@@ -94,7 +94,7 @@ struct Args {
     int ragged;                        // GS_GROUP_N / GS_GROUP_K, -1 = dense
     const int32_t *offsets;
     int split;                         // cluster CTAs sharing a tile's K blocks (1 = none)
-    long long total_tiles;             // dense and ragged K
+    uint32_t total_tiles;              // dense and ragged K
     uint32_t idesc;
     void *C;
     long long ldc, stride_c;
@@ -115,11 +115,11 @@ struct Item {
 constexpr int RASTER = 8;  // rows of tiles visited together, so that concurrent tiles share operands in L2
 
 template <int CG, int BN>
-__device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, const int *off, long long t, uint32_t rank,
+__device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, const int *off, uint32_t t, uint32_t rank,
                                         Item &it) {
     using C_ = Cfg<CG, BN>;
     int p_blocks = a.p_blocks, q_blocks = a.q_blocks, p_base = 0, q_base = 0;
-    long long r = t;
+    uint32_t r = t;
     it.g = 0;
     it.bad = false;
     it.kb0 = 0;
@@ -127,15 +127,15 @@ __device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, co
     it.p_end = a.p.extent;
     it.q_end = a.q.extent;
     if (a.ragged == GS_GROUP_N) {
-        if (t >= tile_start[a.groups]) return false;
+        if (t >= static_cast<uint32_t>(tile_start[a.groups])) return false;
         int lo = 0, hi = a.groups;  // the last group whose first tile is <= t
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (tile_start[mid] <= t) lo = mid;
+            if (static_cast<uint32_t>(tile_start[mid]) <= t) lo = mid;
             else hi = mid;
         }
         it.g = lo;
-        r = t - tile_start[lo];
+        r = t - static_cast<uint32_t>(tile_start[lo]);
         if (C_::WIDE) {
             p_base = off[lo];
             it.p_end = off[lo + 1];
@@ -148,9 +148,9 @@ __device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, co
     } else {
         if (t >= a.total_tiles) return false;
         if (a.ragged == GS_GROUP_K) {
-            const long long per = static_cast<long long>(p_blocks) * q_blocks;
-            it.g = static_cast<int>(t / per);
-            r = t - it.g * per;
+            const uint32_t per = static_cast<uint32_t>(p_blocks) * static_cast<uint32_t>(q_blocks), g = t / per;
+            it.g = static_cast<int>(g);
+            r = t - g * per;
             const int k_lo = off[it.g], k_hi = off[it.g + 1];
             it.kb0 = k_lo / BK;
             it.nkb = (k_hi - k_lo + BK - 1) / BK;
@@ -158,17 +158,18 @@ __device__ __forceinline__ bool item_at(const Args &a, const int *tile_start, co
             if (it.bad) it.nkb = 0;
         }
     }
+    // Tile counts fit 32 bits (checked on entry): every warp of a role works this out for every tile, and 64-bit
+    // divisions here cost the promoters a microsecond a tile.
     const int height = p_blocks < RASTER ? p_blocks : RASTER;
-    const long long span = static_cast<long long>(height) * q_blocks;
-    const int gi = static_cast<int>(r / span);
+    const uint32_t span = static_cast<uint32_t>(height) * static_cast<uint32_t>(q_blocks), gi = r / span;
     const int within = static_cast<int>(r - gi * span);
-    const int first = gi * height;
+    const int first = static_cast<int>(gi) * height;
     const int rows = min(height, p_blocks - first);
-    it.p0 = p_base + (first + within % rows) * C_::TILE_P + static_cast<int>(CG == 2 ? rank : 0) * BM;
-    it.q0 = q_base + within / rows * BN;
+    const int column = within / rows;
+    it.p0 = p_base + (first + within - column * rows) * C_::TILE_P + static_cast<int>(CG == 2 ? rank : 0) * BM;
+    it.q0 = q_base + column * BN;
     if (CG == 1 && a.split > 1) {  // this CTA's share of the K blocks
-        const int lo = static_cast<int>(static_cast<long long>(it.nkb) * rank / a.split);
-        const int hi = static_cast<int>(static_cast<long long>(it.nkb) * (rank + 1) / a.split);
+        const int lo = it.nkb * static_cast<int>(rank) / a.split, hi = it.nkb * static_cast<int>(rank + 1) / a.split;
         it.kb0 += lo;
         it.nkb = hi - lo;
     }
@@ -436,8 +437,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     grid_dep_launch();  // after this CTA has its TMEM: a dependent kernel's CTA cannot take it first
     const uint32_t tmem_base = *tmem_holder;
 
-    const long long tile0 = blockIdx.x / (CG * (CG == 1 ? args.split : 1));
-    const long long tile_step = gridDim.x / (CG * (CG == 1 ? args.split : 1));
+    const uint32_t tile0 = blockIdx.x / (CG * (CG == 1 ? args.split : 1));
+    const uint32_t tile_step = gridDim.x / (CG * (CG == 1 ? args.split : 1));
     Item it;
 
     if (warp < 4) {
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
+            for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
                 const int qc = it.q0 + static_cast<int>(CG == 2 ? rank : 0) * C_::Q_ROWS;
                 const int gp = args.p.grouped ? it.g : 0, gq = args.q.grouped ? it.g : 0;
                 for (int kb = 0; kb < it.nkb; ++kb) {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
             int stage = 0, slot = 0;
             uint32_t phase = 0, sphase = 0;
             bool ok = true;
-            for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
+            for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
 #pragma unroll 1
                 for (int kb = 0; kb < it.nkb; ++kb) {
                     if (!__all_sync(0xffffffffu, mbar_wait2(&tempty[slot], sphase ^ 1u, 2, &full[stage], phase, 3, args.err,
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         int ss = 0;
         uint32_t sp = 0;
         bool ok = true;
-        for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
+        for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
             // This lane's first scale of either side (a scale per vector has its non-K index contiguous), and which of its
             // copies lie inside. What is not copied scales rows and columns that are not stored.
             constexpr int NP = P_VEC ? BM / 32 : 1, NQ = Q_VEC ? BN / 32 : 1;
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         int slot = 0, ss = 0;
         uint32_t phase = 0, sp = 0;
         bool ok = true;
-        for (long long t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
+        for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
             if (it.bad) {
                 if (ew == 0 && lane == 0) atomicOr(args.err, 2u);
                 continue;
@@ -895,7 +896,7 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     const long long tile_n = wide ? BM * t.cg : t.bn, across = wide ? a.q_blocks : a.p_blocks;
     const long long tiles = ragged_n ? across * (d.n / tile_n + (d.groups < d.n ? d.groups : d.n))
                                      : static_cast<long long>(a.p_blocks) * a.q_blocks * (ragged_k ? d.groups : 1);
-    a.total_tiles = tiles;
+    a.total_tiles = static_cast<uint32_t>(tiles);
     const uint32_t p_e5m2 = wide ? d.b_e5m2 : d.a_e5m2, q_e5m2 = wide ? d.a_e5m2 : d.b_e5m2;
     a.idesc = (1u << 4) | (p_e5m2 << 7) | (q_e5m2 << 10) | (static_cast<uint32_t>(a.p.mn) << 15) |
               (static_cast<uint32_t>(a.q.mn) << 16) | ((static_cast<uint32_t>(t.bn) >> 3) << 17) |
