@@ -204,55 +204,64 @@ __device__ __forceinline__ Raw<T> load_raw(const T *col, int r, int rows) {
     return load_part<T>(col, r, rows);
 }
 
-// Vectors down the columns: 16 lanes hold one vector of 128 rows. `lanes` (16 to 256) threads of a block take a
-// column, DEPTH vectors of each thread's on their way at once.
+// Vectors down the columns: 8 lanes hold one vector of 128 rows, each rows 8 s .. and 64 + 8 s .. of it (so that what the
+// lanes of a vector share -- the maximum's last steps, the scale, the addresses -- is spread over 16 elements a lane).
+// `lanes` (8 to 256) threads of a block take a column, DEPTH vectors of each on their way at once.
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(256, 5) k_quant_down(const QuantDesc d, int lanes) {
-    constexpr int DEPTH = sizeof(T) == 4 ? 2 : 4;
+__global__ void __launch_bounds__(256, 4) k_quant_down(const QuantDesc d, int lanes) {
+    constexpr int DEPTH = sizeof(T) == 4 ? 1 : 2;
     grid_dep_wait();
     grid_dep_launch();
-    const int sub = threadIdx.x & 15, per = 256 / lanes;  // columns a block takes at once
-    const uint32_t half = 0xffffu << (threadIdx.x & 16);
+    const int sub = threadIdx.x & 7, per = 256 / lanes;  // columns a block takes at once
+    const uint32_t mates = 0xffu << (threadIdx.x & 24);
+    const int first = (threadIdx.x % lanes) / 8 * 128 + sub * 8, step = lanes * 16;
+    const long long sc_step = static_cast<long long>(step / 128) * d.ld_scale;
     for (long long c = static_cast<long long>(blockIdx.x) * per + threadIdx.x / lanes; c < d.cols; c += static_cast<long long>(gridDim.x) * per) {
         const T *src = source<T>(d, static_cast<int>(c));
         uint8_t *dst = static_cast<uint8_t *>(d.dst) + c * d.ld_dst;
-        const int first = (threadIdx.x % lanes) * 8, step = lanes * 8;
         float *sc = d.scale + c + static_cast<long long>(first / 128) * d.ld_scale;
-        const long long sc_step = static_cast<long long>(step / 128) * d.ld_scale;
         for (int r0 = first; r0 - sub * 8 < d.rows; r0 += DEPTH * step) {
-            Raw<T> raw[DEPTH];
+            Raw<T> raw[DEPTH][2];
             // Whole vectors in all steps: no branch between the loads.
             const bool whole = VEC && src != nullptr && r0 - sub * 8 + (DEPTH - 1) * step + 128 <= d.rows;
             if (whole) {
 #pragma unroll
-                for (int i = 0; i < DEPTH; ++i) raw[i] = load_whole<T>(src + r0 + i * step);
+                for (int i = 0; i < DEPTH; ++i) {
+                    raw[i][0] = load_whole<T>(src + r0 + i * step);
+                    raw[i][1] = load_whole<T>(src + r0 + i * step + 64);
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < DEPTH; ++i) {
-                    const int r = r0 + i * step;
-                    raw[i] = src != nullptr && r < d.rows ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
-                }
+                for (int i = 0; i < DEPTH; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = r0 + i * step + 64 * h;
+                        raw[i][h] = src != nullptr && r < d.rows ? load_raw<T, VEC>(src, r, d.rows) : zero_raw<T>();
+                    }
             }
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i) {
                 const int r = r0 + i * step;
-                if (!whole && r - sub * 8 >= d.rows) break;  // the same answer in all 16 lanes
-                uint32_t top = top_bits(raw[i]);
+                if (!whole && r - sub * 8 >= d.rows) break;  // the same answer in all 8 lanes
+                uint32_t top = max(top_bits(raw[i][0]), top_bits(raw[i][1]));
 #pragma unroll
-                for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
+                for (int s = 4; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(mates, top, s));
                 const bool odd = top >= kInf;
                 if (odd) {
-                    top = finite_top(raw[i]);
+                    top = max(finite_top(raw[i][0]), finite_top(raw[i][1]));
 #pragma unroll
-                    for (int s = 8; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(half, top, s));
+                    for (int s = 4; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(mates, top, s));
                 }
                 const int e = scale_exp<E5M2>(top);
                 if (sub == 0) *sc = pow2(e);
                 sc += sc_step;
                 const float inv[1] = {pow2(-e)};
-                const uint2 q = cast8<T, E5M2>(raw[i], inv, odd);
-                if (whole) *reinterpret_cast<uint2 *>(dst + r) = q;
-                else if (r < d.rows) store8<VEC>(dst, r, d.rows, q);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint2 q = cast8<T, E5M2>(raw[i][h], inv, odd);
+                    if (whole) *reinterpret_cast<uint2 *>(dst + r + 64 * h) = q;
+                    else if (r + 64 * h < d.rows) store8<VEC>(dst, r + 64 * h, d.rows, q);
+                }
             }
         }
     }
@@ -364,9 +373,9 @@ template <typename T, bool E5M2, bool VEC>
 static cudaError_t launch(Context &ctx, const QuantDesc &d) {
     cudaError_t e;
     if (!d.blk && d.axis == 0) {
-        const int depth = sizeof(T) == 4 ? 2 : 4;  // vectors a thread has on their way at once
-        int lanes = 16;
-        while (lanes < 256 && lanes * 8 * depth < d.rows) lanes *= 2;
+        const int depth = sizeof(T) == 4 ? 1 : 2;  // the kernel's DEPTH
+        int lanes = 8;
+        while (lanes < 256 && lanes * 16 * depth < d.rows) lanes *= 2;
         const long long blocks = (static_cast<long long>(d.cols) * lanes + 255) / 256, most = 64LL * ctx.sm_count;
         e = launch_pdl(k_quant_down<T, E5M2, VEC>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d, lanes);
     } else {

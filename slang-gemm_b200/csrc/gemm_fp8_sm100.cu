@@ -66,9 +66,10 @@ struct Cfg {
     static constexpr int P_STAGE = BM * BK;
     static constexpr int Q_STAGE = Q_ROWS * BK;
     static constexpr int STAGE = P_STAGE + Q_STAGE;
-    static constexpr int STAGES = WIDE ? (CG == 2 ? 5 : 3) : (STAGE >= 32 * 1024 ? 6 : 8);
+    static constexpr int STAGES = WIDE ? 4 : (STAGE >= 32 * 1024 ? 6 : 8);
+    static_assert(!WIDE || CG == 2, "the wide tile is a CTA-pair tile");
     static constexpr int STG_BLOCK = 32 * 128;  // a promoter warp's staging: 32 rows of 128 bytes
-    static constexpr int STG_BYTES = WIDE ? EPI_WARPS * STG_BLOCK : 0;
+    static constexpr int STG_BYTES = WIDE ? 2 * EPI_WARPS * STG_BLOCK : 0;  // two to a warp
     static constexpr int SLOTS = BN == 256 ? 2 : 4;
     static constexpr int TMEM_COLS = BN * SLOTS;
     static constexpr int SC_FLOATS = BN + BM;
@@ -469,13 +470,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                         mbar_arrive_expect_tx(&full[stage], C_::STAGE);
                         if (args.p.mn) tma_load_3d_hint(dP, &tmP, &full[stage], it.p0, k0, gp, pol);
                         else tma_load_3d_hint(dP, &tmP, &full[stage], k0, it.p0, gp, pol);
-                        if (args.q.mn) {  // only with BN >= 128: panels of 128 columns
-#pragma unroll
-                            for (int c = 0; c < (BN + 127) / 128; ++c)
-                                tma_load_3d_hint(dQ + c * 128 * BK, &tmQ, &full[stage], qc + c * 128, k0, gq, pol);
-                        } else {
-                            tma_load_3d_hint(dQ, &tmQ, &full[stage], k0, qc, gq, pol);
-                        }
+                        if (args.q.mn) tma_load_3d_hint(dQ, &tmQ, &full[stage], qc, k0, gq, pol);  // only with BN = 128
+                        else tma_load_3d_hint(dQ, &tmQ, &full[stage], k0, qc, gq, pol);
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -646,8 +642,6 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                     for (int j = 0; j < 64; ++j) acc[j] = mul2(acc[j], al);
                 }
                 if (args.tma_store && (args.ragged != GS_GROUP_N || p_warp + 32 <= it.p_end)) {
-                    uint8_t *buf = stg + ew * C_::STG_BLOCK;
-                    const uint32_t dst = smem_u32(buf) + lane * 128;
                     const int gc = args.ragged == GS_GROUP_K ? it.g : 0;
                     // `words` packs the 16 bytes of chunk x of block b
                     auto blocks = [&](auto cols_c, auto words) {
@@ -655,7 +649,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
 #pragma unroll
                         for (int b = 0; b < 128 / COLS; ++b) {
                             if (b * COLS >= n || p_warp >= it.p_end) break;
-                            if (lane == 0) bulk_wait_group_read<0>();
+                            if (lane == 0) bulk_wait_group_read<1>();  // of the store that last used this buffer
+                            uint8_t *buf = stg + (ew * 2 + (b & 1)) * C_::STG_BLOCK;
+                            const uint32_t dst = smem_u32(buf) + lane * 128;
                             __syncwarp();
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
@@ -943,7 +939,6 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     const int mode = (p_vec ? 1 : 0) | (q_vec ? 2 : 0);
     ctx.last_kernels |= GS_KERNEL_TC_F8;
     if (t.cg == 2) return launch_mode<2, 256>(ctx, mode, maps, a, tiles);
-    if (t.bn == 256) return launch_mode<1, 256>(ctx, mode, maps, a, tiles);
     if (t.bn == 128) return launch_mode<1, 128>(ctx, mode, maps, a, tiles);
     if (t.bn == 64) return launch_mode<1, 64>(ctx, mode, maps, a, tiles);
     return launch_mode<1, 32>(ctx, mode, maps, a, tiles);

@@ -87,30 +87,53 @@ __global__ void __launch_bounds__(256) k_combine(const CombineDesc d, int lanes)
     }
 }
 
-// A block handles one row of y: its dy, and its slot's weight gradient.
+// A warp handles one row of y: its dy, and its slot's weight gradient; four steps of 256 columns on their way at once.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_combine_backward(const CombineDesc d) {
-    __shared__ float part[8];
+    constexpr int DEPTH = sizeof(T) == 4 ? 2 : 4;
     grid_dep_wait();
     grid_dep_launch();
+    const int lane = threadIdx.x & 31;
     const long long slots = static_cast<long long>(d.tokens) * d.top_k;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < slots; i += gridDim.x * 256LL) {
         const int r = d.slot_row[i];
         if (r < 0 || r >= d.rows) d.dweights[i] = 0.0f;  // a slot without a row
     }
-    for (long long r = blockIdx.x; r < d.rows; r += gridDim.x) {
+    for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < d.rows; r += gridDim.x * 8LL) {
         const int slot = d.row_slot[r];
         T *dy = static_cast<T *>(d.dy) + r * d.lddy;
         if (slot < 0 || slot >= slots) {
             const float zero[V] = {};
-            for (int h = threadIdx.x * V; h < d.hidden; h += 256 * V) store8<T, VEC>(dy, h, d.hidden, zero);
+            for (int h = lane * V; h < d.hidden; h += 32 * V) store8<T, VEC>(dy, h, d.hidden, zero);
             continue;
         }
         const float w = d.weights[slot];
         const T *y = static_cast<const T *>(d.y) + r * d.ldy;
         const T *g = static_cast<const T *>(d.dout) + static_cast<long long>(slot / d.top_k) * d.lddo;
         float dot = 0.0f;
-        for (int h = threadIdx.x * V; h < d.hidden; h += 256 * V) {
+        int h = lane * V;
+        if (VEC) {
+            for (; h - lane * V + DEPTH * 32 * V <= d.hidden; h += DEPTH * 32 * V) {
+                Pack<T, V> a[DEPTH], b[DEPTH];
+#pragma unroll
+                for (int i = 0; i < DEPTH; ++i) {
+                    a[i] = load_pack<T, V>(g + h + i * 32 * V);
+                    b[i] = load_pack<T, V>(y + h + i * 32 * V);
+                }
+#pragma unroll
+                for (int i = 0; i < DEPTH; ++i) {
+                    Pack<T, V> o;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float x = to_f32(a[i].v[v]);
+                        dot = fmaf(x, to_f32(b[i].v[v]), dot);
+                        o.v[v] = from_f32<T>(w * x);
+                    }
+                    store_pack<T, V>(dy + h + i * 32 * V, o);
+                }
+            }
+        }
+        for (; h < d.hidden; h += 32 * V) {
             float a[V], b[V], o[V];
             load8<T, VEC>(g, h, d.hidden, a);
             load8<T, VEC>(y, h, d.hidden, b);
@@ -123,15 +146,7 @@ __global__ void __launch_bounds__(256) k_combine_backward(const CombineDesc d) {
         }
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum += part[k];
-            d.dweights[slot] = sum;
-        }
-        __syncthreads();
+        if (lane == 0) d.dweights[slot] = dot;
     }
 }
 
@@ -162,8 +177,8 @@ cudaError_t launch_combine(Context &ctx, const CombineDesc &d) {
 
 cudaError_t launch_combine_backward(Context &ctx, const CombineDesc &d) {
     ctx.last_kernels |= GS_KERNEL_COMBINE;
-    const long long most = 64LL * ctx.sm_count;
-    const unsigned blocks = static_cast<unsigned>(d.rows < 1 ? 1 : d.rows < most ? d.rows : most);
+    const long long want = (static_cast<long long>(d.rows) + 7) / 8, most = 32LL * ctx.sm_count;
+    const unsigned blocks = static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
     return with_float_type(d.type, [&](auto z) {
         using T = decltype(z);
         const bool vec = combine::aligned(d.y, d.ldy, sizeof(T)) && combine::aligned(d.dout, d.lddo, sizeof(T)) &&

@@ -334,7 +334,9 @@ def test_combine_backward(handle, t, k, hidden, dtype, pad):
     assert bool((dy[:, hidden:] == 7).all())
     mag = (torch.where(live[:, :, None], y[:, :hidden].double()[slot_row.clamp(min=0).long()], 0.0).abs() *
            dout[:, None, :hidden].double().abs()).sum(2)
-    terms = hidden / 256 + 8 + 13  # of one thread, then 5 shuffles and 8 warps
+    # a lane's chain of fused multiply-adds (8 of every 256 columns, rounded up), then 5 shuffles, each half a step of at
+    # most the sum of magnitudes
+    terms = -(-hidden // 256) * 8 + 5
     assert bool(((dw.double().cpu() - lw.grad).abs() <= terms * 2.0 ** -24 * mag).all())
 
 
