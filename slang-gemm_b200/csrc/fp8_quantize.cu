@@ -374,8 +374,11 @@ static cudaError_t launch(Context &ctx, const QuantDesc &d) {
     cudaError_t e;
     if (!d.blk && d.axis == 0) {
         const int depth = sizeof(T) == 4 ? 1 : 2;  // the kernel's DEPTH
+        // A warp a column (finding the source column then costs little); more threads where columns are few, fewer where
+        // they are short.
         int lanes = 8;
-        while (lanes < 256 && lanes * 16 * depth < d.rows) lanes *= 2;
+        while (lanes < 256 && lanes * 16 * depth < d.rows && (lanes < 32 || static_cast<long long>(d.cols) * lanes < 2048LL * ctx.sm_count))
+            lanes *= 2;
         const long long blocks = (static_cast<long long>(d.cols) * lanes + 255) / 256, most = 64LL * ctx.sm_count;
         e = launch_pdl(k_quant_down<T, E5M2, VEC>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, 1, d, lanes);
     } else {
