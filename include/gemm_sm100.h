@@ -340,8 +340,9 @@ gs_status gs_gemm_fp8_grouped(gs_handle handle, int ragged, int transa, int tran
 
 /* The tile a gs_gemm_fp8 (groups = 0) or gs_gemm_fp8_grouped call would use on
  * a device with sm_count SMs: *columns per tile, *ctas (1 = 128 rows, 2 = a pair
- * with 256) and *k_slices (CTAs of a cluster that share a tile's K). Pure host
- * logic, for tests and capacity planning. */
+ * with 256) and *k_slices (CTAs of a cluster that share a tile's K), for A in
+ * BLK128, B in VEC128 and a 16-byte aligned 16-bit C. Pure host logic, for tests
+ * and capacity planning. */
 gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int k, int groups, int sm_count, int *columns,
                            int *ctas, int *k_slices);
 

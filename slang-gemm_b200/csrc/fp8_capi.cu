@@ -263,6 +263,8 @@ gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int
     d.k = k;
     d.groups = groups;
     d.ragged = ragged;
+    d.b_vec = 1;
+    d.out_kind = OUT_BF16;
     const fp8::Tile t = fp8::choose_tile(d, sm_count);
     *columns = t.bn;
     *ctas = t.cg;

@@ -250,9 +250,12 @@ __device__ __forceinline__ float4 ld_shared_f32x4(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -769,16 +772,26 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
             uint32_t base[MAX_SPLIT];
 #pragma unroll
             for (int x = 0; x < MAX_SPLIT; ++x) base[x] = mapa_shared(smem_u32(smem), static_cast<uint32_t>(min(x, args.split - 1)));
-            for (int e = first * BM + static_cast<int>(threadIdx.x); e < last * BM; e += C_::THREADS) {
-                const int p = it.p0 + e % BM;
+            // Four consecutive rows a thread.
+            for (int e = first * (BM / 4) + static_cast<int>(threadIdx.x); e < last * (BM / 4); e += C_::THREADS) {
+                const int p = it.p0 + e % (BM / 4) * 4;
                 if (p >= it.p_end) continue;
-                float v[MAX_SPLIT];
+                float4 v[MAX_SPLIT];
 #pragma unroll
-                for (int x = 0; x < MAX_SPLIT; ++x) v[x] = x < args.split ? ld_cluster_f32(base[x] + e * 4) : 0.0f;
-                float sum = v[0];
+                for (int x = 0; x < MAX_SPLIT; ++x) v[x] = x < args.split ? ld_cluster_f32x4(base[x] + e * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float4 sum = v[0];
 #pragma unroll
-                for (int x = 1; x < MAX_SPLIT; ++x) sum = __fadd_rn(sum, v[x]);
-                store_c(args, Cb, static_cast<size_t>(p) + static_cast<size_t>(it.q0 + e / BM) * args.ldc, sum);
+                for (int x = 1; x < MAX_SPLIT; ++x) {
+                    sum.x = __fadd_rn(sum.x, v[x].x);
+                    sum.y = __fadd_rn(sum.y, v[x].y);
+                    sum.z = __fadd_rn(sum.z, v[x].z);
+                    sum.w = __fadd_rn(sum.w, v[x].w);
+                }
+                const size_t i = static_cast<size_t>(p) + static_cast<size_t>(it.q0 + e / (BM / 4)) * args.ldc;
+                store_c(args, Cb, i, sum.x);
+                if (p + 1 < it.p_end) store_c(args, Cb, i + 1, sum.y);
+                if (p + 2 < it.p_end) store_c(args, Cb, i + 2, sum.z);
+                if (p + 3 < it.p_end) store_c(args, Cb, i + 3, sum.w);
             }
         }
         __syncwarp();
@@ -858,26 +871,54 @@ static cudaError_t launch_mode(Context &ctx, int mode, const Maps &maps, const A
 
 static int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Tile of a product: bn columns, cg CTAs, split K slices.
+// C's rows can be moved 16 bytes at a time.
+static bool aligned_c(const GemmFp8Desc &d) {
+    const size_t es = out_elem_size(d.out_kind);
+    const bool many = d.groups > 1 && d.ragged == GS_GROUP_K;
+    return reinterpret_cast<uintptr_t>(d.C) % 16 == 0 && d.ldc * es % 16 == 0 && (!many || d.stride_c * es % 16 == 0);
+}
+
+// Tile of a product: bn columns, cg CTAs, split K slices. Each kind of tile is given the microseconds that its K blocks
+// and the rest of it took in a sweep of 13 shapes from 512^3 to 8192^3, dense and ragged, alone on the GPU (a pair's 256 x 256
+// tile 0.50 a K block, 0.86 with a scale per row and per column; 128 x 128, 64 and 32 tiles of one SM 0.41, 0.30 and
+// 0.25); the cheapest rounds-times-tile wins. Against a rule on the column count alone: 1024^3 12.5 -> 6.9 us, 1024 x 1024 x 4096
+// with both scales per vector 32 -> 17 us, 64 groups of 32 rows 82 -> 53 us.
+// Narrow tiles that leave SMs without work may share their K blocks over a cluster, as long as all clusters run at once
+// (4096 x 16 x 4096, 32 tiles as 128 CTAs: 11.7 -> 8.6 us; clusters of eight do not pack a GPU that is nearly full).
 Tile choose_tile(const GemmFp8Desc &d, int sm_count) {
-    Tile t{1, 256, 1};
-    // Columns of C a tile can expect to fill: a ragged group's mean share, or all of them.
     const bool ragged_n = d.groups > 0 && d.ragged == GS_GROUP_N, ragged_k = d.groups > 0 && d.ragged == GS_GROUP_K;
-    const long long cols = ragged_n ? cdiv(d.n, d.groups) : d.n;
-    if (cols <= 32 && !d.trans_b) t.bn = 32;
-    else if (cols <= 64 && !d.trans_b) t.bn = 64;
-    else if (cols <= 128) t.bn = 128;
-    else t.cg = 2;
-    // Narrow tiles that leave SMs without work share their K blocks over a cluster, two K blocks or more to a CTA, as
-    // long as all clusters run at once. (4096 x 16 x 4096: 32 tiles of 32 K blocks, as 128 CTAs 18.4 -> 7.0 us.)
-    if (t.bn < 256) {
-        const long long tiles = static_cast<long long>(cdiv(d.m, BM)) *
-                                (ragged_n ? d.n / t.bn + (d.groups < d.n ? d.groups : d.n)
-                                          : static_cast<long long>(cdiv(d.n, t.bn)) * (ragged_k ? d.groups : 1));
-        const int kb = ragged_k ? cdiv(cdiv(d.k, BK), d.groups) : cdiv(d.k, BK);
-        while (t.split < MAX_SPLIT && tiles * t.split * 2 <= sm_count && kb >= 4 * t.split) t.split *= 2;
+    const double kb = ragged_k ? static_cast<double>(d.k) / BK / d.groups : static_cast<double>(cdiv(d.k, BK));
+    const double live = ragged_n ? (d.groups < d.n ? d.groups : d.n) : 0;  // groups that can hold a column
+    const bool f32_out = d.out_kind == OUT_F32;
+    struct Kind { int bn; double per_kb, rest, part; };  // part: the share of a tile a ragged group wastes
+    const Kind kinds[4] = {{32, 0.25, 1.1, 0.5},
+                           {64, 0.30, 1.25, 0.5},
+                           {128, 0.41, 1.7, 0.5},
+                           {256, d.a_vec ? (d.b_vec ? 0.86 : 0.75) : 0.50, !aligned_c(d) ? 20.0 : f32_out ? 4.0 : 2.0, 0.75}};
+    Tile best{2, 256, 1};
+    double least = 1e300;
+    for (const Kind &kind : kinds) {
+        if (d.trans_b && kind.bn < 128) continue;  // op(B) = T is read in panels of 128 columns
+        const bool wide = kind.bn == 256;
+        const double across = cdiv(d.m, wide ? kind.bn : BM);
+        double along = ragged_n ? static_cast<double>(d.n) / kind.bn + kind.part * live : static_cast<double>(cdiv(d.n, kind.bn));
+        if (ragged_n && along < live) along = live;
+        const double tiles = across * along * (ragged_k ? d.groups : 1);
+        const double at_once = wide ? (sm_count > 1 ? sm_count / 2 : 1) : sm_count;
+        // the launch must hold every cluster: count the tiles as it does
+        const double most = ragged_n ? across * (d.n / kind.bn + live) : tiles;
+        for (int split = 1; split <= (wide ? 1 : MAX_SPLIT); split *= 2) {
+            if (split > 1 && (kb < 2 * split || most * split > (split == 8 ? 96.0 : split == 4 ? 132.0 : 148.0) * sm_count / 148.0)) break;
+            double rounds = tiles * split / at_once;
+            rounds = rounds <= 1.0 ? 1.0 : static_cast<double>(static_cast<long long>(rounds + 0.999));
+            const double cost = rounds * (kb / split * kind.per_kb + kind.rest) + (split > 1 ? 1.0 + 0.025 * kind.bn : 0.0);
+            if (cost < least) {
+                least = cost;
+                best = Tile{wide ? 2 : 1, kind.bn, split};
+            }
+        }
     }
-    return t;
+    return best;
 }
 
 }  // namespace fp8
@@ -929,7 +970,7 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     a.err = ctx.dev_err;
     a.spin_limit = ctx.spin_limit;
     const size_t es = out_elem_size(d.out_kind);
-    a.vec_c = reinterpret_cast<uintptr_t>(d.C) % 16 == 0 && d.ldc * es % 16 == 0 && (!ragged_k || d.groups == 1 || d.stride_c * es % 16 == 0);
+    a.vec_c = aligned_c(d) ? 1 : 0;
 
     Maps maps{};
     std::string why;

@@ -171,7 +171,9 @@ def test_plan_rows_and_workspace_refusals():
 def test_plan_tile():
     s, bn, cg, parts = gs.plan_gemm_fp8(1, 0, 8192, 8192, 8192)
     assert (s, bn, cg, parts) == (0, 256, 2, 1)
-    assert gs.plan_gemm_fp8(1, 0, 4096, 16, 4096)[1] == 32
+    assert gs.plan_gemm_fp8(1, 0, 4096, 16, 4096) == (0, 32, 1, 4)      # few tokens: narrow tiles, K over clusters
+    assert gs.plan_gemm_fp8(1, 0, 1024, 16, 8192) == (0, 32, 1, 8)
+    assert gs.plan_gemm_fp8(1, 0, 1024, 1024, 1024) == (0, 64, 1, 1)    # 128 tiles for 148 SMs instead of 16 pair tiles
     assert gs.plan_gemm_fp8(0, 1, 4096, 16, 4096)[1] == 128  # op(B) = T is read in panels of 128 columns
     assert gs.plan_gemm_fp8(1, 0, 2048, 128, 2048, groups=64)[1:] == (32, 1, 1)
     for bad in (dict(m=0, n=1, k=1), dict(m=1, n=1, k=1, groups=gs.FP8_MAX_GROUPS + 1), dict(m=1, n=1, k=1, groups=1, ragged=5)):
