@@ -105,6 +105,7 @@ struct Args {
     Epilogue ep;
     uint32_t *err;
     long long spin_limit;
+    int debug_skip_kb;                 // test hook (>= 0): the producer leaves this K block of its first tile out, then stops
 };
 
 // A tile of group g: rows p0.. (p_end: behind the last), columns q0.., K blocks kb0..kb0+nkb.
@@ -481,12 +482,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         if (lane == 0) {
             const uint64_t pol = l2_policy_evict_normal();
             int stage = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 0, issued = 0;
             bool ok = true;
             for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
                 const int qc = it.q0 + static_cast<int>(CG == 2 ? rank : 0) * C_::Q_ROWS;
                 const int gp = args.p.grouped ? it.g : 0, gq = args.q.grouped ? it.g : 0;
                 for (int kb = 0; kb < it.nkb; ++kb) {
+                    if (kb == args.debug_skip_kb && t == tile0) { ok = false; break; }
                     if (!mbar_wait(&empty[stage], phase ^ 1u, args.err, 1, args.spin_limit)) { ok = false; break; }
                     uint8_t *dP = smP + stage * C_::P_STAGE;
                     uint8_t *dQ = smQ + stage * C_::Q_STAGE;
@@ -505,9 +507,15 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                         if (args.q.mn) tma_load_3d_hint(dQ, &tmQ, &full[stage], qc, k0, gq, pol);  // only with BN = 128
                         else tma_load_3d_hint(dQ, &tmQ, &full[stage], k0, qc, gq, pol);
                     }
+                    ++issued;
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
+            // Giving up: the copies still in flight (a pair's: both CTAs' complete on the even one's barriers) land before
+            // the CTA goes.
+            if (!ok && leader)
+                for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+                    mbar_wait(&full[i % STAGES], (i / STAGES) & 1u, args.err, 8, args.spin_limit);
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (even CTA) ----------------
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
         bool ok = true;
         for (uint32_t t = tile0; ok && item_at<CG, BN>(args, tile_start, off, t, rank, it); t += tile_step) {
             if (it.bad) {
-                if (ew == 0 && lane == 0) atomicOr(args.err, 2u);
+                if (ew == 0 && lane == 0) atomicOr(args.err, GS_DEVERR_OFFSETS);
                 continue;
             }
             uint64_t acc[EPI_COLS / 2];
@@ -969,6 +977,7 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     a.ep = d.ep;
     a.err = ctx.dev_err;
     a.spin_limit = ctx.spin_limit;
+    a.debug_skip_kb = ctx.debug_skip_kb;
     const size_t es = out_elem_size(d.out_kind);
     a.vec_c = aligned_c(d) ? 1 : 0;
 

@@ -12,9 +12,11 @@
 
 namespace gs {
 
-// Device error word layout: bit 0 = a wait timed out; bits 8..15 = site code
-// of the first timeout.
+// Device error word layout: bit 0 = a wait timed out; bit 1 = a ragged FP8
+// product left out a group whose offsets are not whole K blocks; bits 8..15 =
+// site code of the first timeout.
 constexpr uint32_t GS_DEVERR_TIMEOUT = 1u;
+constexpr uint32_t GS_DEVERR_OFFSETS = 2u;
 // Suspend-time hint of one try_wait, in ns: a waiting thread sleeps until the
 // phase completes or this much time has passed, instead of re-polling.
 constexpr uint32_t kTryWaitHintNs = 1000000;
@@ -82,7 +84,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32
     while (true) {
         if (mbar_try_wait_hint(addr, parity, kTryWaitHintNs)) return true;
         if (clock64() - start > limit) {
-            if (err) atomicCAS(err, 0u, GS_DEVERR_TIMEOUT | (site << 8));
+            if (err && atomicCAS(err, 0u, GS_DEVERR_TIMEOUT | (site << 8)) == GS_DEVERR_OFFSETS)
+                atomicCAS(err, GS_DEVERR_OFFSETS, GS_DEVERR_OFFSETS | GS_DEVERR_TIMEOUT | (site << 8));
             return false;
         }
     }

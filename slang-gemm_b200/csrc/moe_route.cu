@@ -597,46 +597,68 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
 }
 
 // Gradient of the weights with respect to the logits; the choice is constant.
-//   softmax, renormalised: a softmax over the chosen experts alone
-//   otherwise dl = J^T ds, with ds_j = scale * (g_j - sum g w) / S or scale * g_j
+//   renormalised: dl_j = w_j (g_j - sum g w), times 1 - s_j for sigmoid; experts that were not chosen get 0
+//   otherwise dl = J^T g: g_j s_j (1 - s_j), or s_e ([e chosen] g_e - sum g s)
+// Bound by writing dlogits (and, for softmax that is not renormalised, reading the logits).
 template <typename T, typename TD, int VPL>
 __global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ RouteBwdDesc d) {
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
     for (long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < d.tokens; t += static_cast<long long>(gridDim.x) * 8) {
-        float l[VPL], s[VPL];
-        load_row<T, VPL>(static_cast<const T *>(d.logits) + t * d.ld, d.experts, lane, l);
-        scores<false, float, VPL>(l, d.sigmoid != 0, d.sigmoid ? 0.0f : row_top(l), s);
+        const T *logits = static_cast<const T *>(d.logits) + t * d.ld;
         int id = -1;
-        float g = 0.0f;
+        float g = 0.0f, x = -INFINITY;  // lane j: the j-th chosen expert, its weight's gradient and its logit
         if (lane < d.top_k) {
             id = d.ids[t * d.top_k + lane];
-            if (id < 0 || id >= d.experts) id = -1;
-            else g = d.dweights[t * d.top_k + lane] * d.scale;
+            if (id < 0 || id >= d.experts) {
+                id = -1;
+            } else {
+                g = d.dweights[t * d.top_k + lane] * d.scale;
+                x = to_f32(logits[id]);
+                x = x >= -INFINITY ? fminf(x, kTop) : -INFINITY;
+            }
         }
-        float sj = 0.0f, lj = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const float v = __shfl_sync(kFull, s[i], id & 31), x = __shfl_sync(kFull, l[i], id & 31);
-            if (id >= 0 && (id >> 5) == i) { sj = v; lj = x; }
-        }
-        // slope_j: what chosen expert j's own logit gets; common: what every logit gets, times its score (softmax)
-        float slope, common = 0.0f;
+        // slope: what chosen expert j's own logit gets; common: what every logit gets, times its score (softmax that is
+        // not renormalised: the one case that needs the other experts' logits)
+        float s[VPL], slope, common = 0.0f;
         if (d.renorm) {
-            const float sum = warp_sum(sj);
-            const float w = sum > 0.0f ? sj / sum : 0.0f;
-            const float dev = g - warp_sum(g * w);
-            slope = id >= 0 ? w * dev : 0.0f;
-            if (d.sigmoid) slope *= 1.0f / (1.0f + expf(lj));
+            // Weights from the logits' differences, or from the sigmoids unless all of them are below f32's range (where a
+            // sigmoid is an exponential).
+            float v = d.sigmoid ? 1.0f / (1.0f + expf(-x)) : 0.0f;
+            float sum = warp_sum(v);
+            if (!(sum >= 1e-30f)) {
+                const float most = value_of(warp_max(key_of(x)));
+                v = id >= 0 && x > -INFINITY ? expf(x - most) : 0.0f;
+                sum = warp_sum(v);
+            }
+            const float w = sum > 0.0f ? v / sum : 0.0f;
+            slope = w * (g - warp_sum(g * w));
+            if (d.sigmoid) slope *= 1.0f / (1.0f + expf(x));
+        } else if (d.sigmoid) {
+            slope = g / (1.0f + expf(-x)) * (1.0f / (1.0f + expf(x)));
         } else {
-            slope = g * sj;
-            if (d.sigmoid) slope *= 1.0f / (1.0f + expf(lj));
-            else common = warp_sum(slope);
-        }
-        float out[VPL];
+            float l[VPL];
+            load_row<T, VPL>(logits, d.experts, lane, l);
+            const float top = row_top(l);
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) out[i] = -common * s[i];
+            for (int i = 0; i < VPL; ++i) {
+                s[i] = l[i] == -INFINITY ? 0.0f : expf(l[i] - top);
+                sum += s[i];
+            }
+            sum = warp_sum(sum);
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) s[i] *= inv;
+            slope = id >= 0 && x > -INFINITY ? g * (expf(x - top) * inv) : 0.0f;
+            common = warp_sum(slope);
+        }
+        if (id < 0) slope = 0.0f;
+        float out[VPL];
+        const bool every = !d.renorm && !d.sigmoid;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) out[i] = every ? -common * s[i] : 0.0f;
         for (int j = 0; j < d.top_k; ++j) {
             const int e = __shfl_sync(kFull, id, j);
             const float v = __shfl_sync(kFull, slope, j);

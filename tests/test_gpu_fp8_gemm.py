@@ -235,5 +235,46 @@ def test_two_graphs_of_one_handle_run_at_once(cuda):
         del graphs, g
 
 
+@pytest.mark.parametrize("m,n,k,tb,mb", [(2048, 2048, 1024, N, VEC), (4096, 16, 4096, N, VEC), (1024, 512, 1024, N, BLK),
+                                         (256, 4096, 1024, T, VEC)])
+def test_wait_that_runs_out_ends_the_kernel_and_is_reported(cuda, m, n, k, tb, mb):
+    """As test_gpu_wait_limit.py does for the other tensor-core kernels: the producer leaves a K block out (no copy, nothing
+    issued after it), so the waits for it run out after a millisecond; the call is reported and the next one is right."""
+    gen = torch.Generator().manual_seed(m)
+    a, b = operands(gen, T, tb, m, n, k, BLK if tb == N else VEC, mb)
+    with gs.Handle() as h:
+        h.set_wait_limit(2_000_000)
+        h.debug_skip_kblock(1)
+        c = torch.empty(n, m, device="cuda")
+        h.gemm_fp8(T, tb, m, n, k, 1.0, a.bytes, a.type, a.ld, a.scale, a.mode, a.lds, b.bytes, b.type, b.ld, b.scale, b.mode, b.lds,
+                   0.0, c, gs.R_32F, m)
+        word = h.device_error()
+    assert word & 1 and (word >> 8) & 0xFF in (1, 2, 3, 4, 6, 7), hex(word)
+    with gs.Handle() as h:
+        h.set_wait_limit(2_000_000)  # healthy pipelines do not notice it
+        assert torch.equal(run_gemm(h, a, b, T, tb, m, n, k, gs.R_32F).double(), product(a.values(), b.values())[0])
+
+
+@pytest.mark.parametrize("bn,m,n,k,groups", [(32, 4096, 20, 2048, 0), (64, 1024, 1024, 640, 0), (128, 2048, 1024, 2048, 0),
+                                             (256, 2048, 2048, 512, 0), (32, 512, 100, 512, 40), (256, 2048, 8000, 512, 4)])
+def test_every_tile_kind(handle, bn, m, n, k, groups):
+    """One product for each kind of tile, as the plan says, exact on whole numbers."""
+    assert gs.plan_gemm_fp8(T, N, m, n, k, groups=groups)[1] == bn
+    gen = torch.Generator().manual_seed(bn + groups)
+    a, b = operands(gen, T, N, m, n, k, BLK, VEC, batch=max(groups, 1))
+    if not groups:
+        assert torch.equal(run_gemm(handle, a, b, T, N, m, n, k, gs.R_16BF), product(a.values(), b.values())[0].bfloat16())
+        return
+    off = _offsets(gen, groups, n)
+    c = torch.empty(n, m, dtype=torch.bfloat16, device="cuda")
+    handle.gemm_fp8_grouped(gs.GROUP_N, T, N, m, n, k, groups, torch.tensor(off, dtype=torch.int32, device="cuda"), 1.0, a.bytes, E4,
+                            a.ld, a.stride, a.scale, BLK, a.lds, a.stride_s, b.bytes, E4, b.ld, b.scale, VEC, b.lds, 0.0, c,
+                            gs.R_16BF, m, 0)
+    torch.cuda.synchronize()
+    bv = b.values()
+    for g in range(groups):
+        assert torch.equal(c[off[g]:off[g + 1]], product(a.values(g), bv[off[g]:off[g + 1]])[0].bfloat16())
+
+
 def test_scale_matrix_shape_helper():
     assert [blocks(x) for x in (1, 127, 128, 129)] == [1, 1, 1, 2]
