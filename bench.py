@@ -1041,6 +1041,72 @@ def run_tile_sweep(args) -> int:
     return 0
 
 
+# tokens, experts, top_k, d_in, d_out of `--experts`
+EXPERT_SHAPES = [(1, 64, 4, 2048, 2048), (32, 64, 4, 2048, 2048), (512, 64, 4, 2048, 2048), (4096, 32, 4, 4096, 2048),
+                 (16384, 32, 2, 2048, 4096)]
+
+
+def run_experts(args) -> int:
+    """A routed FP8 expert layer (routed_experts.RoutedExperts) forward and, from 512 tokens, with its gradients, each
+    captured into a CUDA graph and replayed after a 256 MiB L2 flush; medians of `--steps` replays. One JSON line per
+    shape, with the products' share of the time's floor at the measured peaks."""
+    import torch
+
+    import gemm_sm100 as gs
+    from routed_experts import RoutedExperts
+
+    torch.cuda.set_device(0)
+    stream = torch.cuda.Stream()
+    flush = torch.empty(256 * 2 ** 20, dtype=torch.uint8, device="cuda")
+    peaks = load_peaks()
+
+    def median_us(graph):
+        times = []
+        for i in range(args.warmup + args.steps):
+            flush.zero_()
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            graph.replay()
+            e1.record()
+            e1.synchronize()
+            if i >= args.warmup:
+                times.append(e0.elapsed_time(e1) * 1e3)
+        return sorted(times)[len(times) // 2]
+
+    with gs.Handle(stream) as h:
+        for tokens, experts, top_k, d_in, d_out in EXPERT_SHAPES:
+            train = tokens >= 512
+            g = torch.Generator(device="cuda").manual_seed(tokens)
+            with torch.cuda.stream(stream):
+                layer = RoutedExperts(h, tokens, experts, top_k, d_in, d_out, align=128 if train else 1)
+                layer.set_weights(torch.randn(experts, d_out, d_in, generator=g, device="cuda") * d_in ** -0.5)
+                x = torch.randn(tokens, d_in, generator=g, device="cuda").to(torch.bfloat16)
+                logits = torch.randn(tokens, experts, generator=g, device="cuda")
+                dout = torch.randn(tokens, d_out, generator=g, device="cuda").to(torch.bfloat16)
+                layer.forward(x, logits)
+                if train:
+                    layer.backward(x, logits, dout)
+            stream.synchronize()
+            fwd, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(fwd, stream=stream):
+                layer.forward(x, logits)
+            line = {"mode": "experts", "tokens": tokens, "experts": experts, "top_k": top_k, "d_in": d_in, "d_out": d_out,
+                    "forward_us": round(median_us(fwd), 2)}
+            flops = 2.0 * tokens * top_k * d_in * d_out
+            live = min(experts, tokens * top_k)
+            floor = max(flops / (2e6 * peaks["bf16"]), live * d_in * d_out / (1e3 * peaks["hbm_gbs"]))
+            line["products_floor_us"] = round(floor, 2)
+            if train:
+                with torch.cuda.graph(both, stream=stream):
+                    layer.forward(x, logits)
+                    layer.backward(x, logits, dout)
+                line["forward_backward_us"] = round(median_us(both), 2)
+            assert h.device_error() == 0
+            emit(line)
+            del fwd, both
+    return 0
+
+
 def main():
     global _RESULT_FD
     sys.stdout.flush()
@@ -1079,6 +1145,8 @@ def main():
                          "cuBLAS over the sweep's shapes ('tiles') or the split-K shapes ('splitk')")
     ap.add_argument("--sweep-shapes", default=None, help="--tile-sweep shapes, MxNxK[xBATCH] comma-separated")
     ap.add_argument("--sweep-dtypes", default="f16,i8", help="--tile-sweep input types: f16, bf16, i8")
+    ap.add_argument("--experts", action="store_true",
+                    help="instead of the contract line: a routed FP8 expert layer, forward and with its gradients")
     rows = ap.add_argument_group("manifest rows (the reference's JSONL benchmark CLI; any of these selects it)")
     rows.add_argument("--manifest", default=None, help="'all': every API/op/type case (bench/gemm_perf.zig:91)")
     rows.add_argument("--sizes", default=None, help="comma-separated square sizes (default 512,1024,2048)")
@@ -1107,6 +1175,8 @@ def main():
         sys.exit(run_manifest(args))
     if args.tile_sweep:
         sys.exit(run_tile_sweep(args))
+    if args.experts:
+        sys.exit(run_experts(args))
     if args.sustained:
         run_sustained(args, args.config)
         return

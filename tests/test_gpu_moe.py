@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import gemm_sm100 as gs
-from fp8_util import FLOAT, blocks
+from fp8_util import FLOAT
+from routed_experts import RoutedExperts
 
 pytestmark = pytest.mark.gpu
 TYPE = {v: k for k, v in FLOAT.items()}
@@ -353,77 +354,11 @@ def test_combine_without_tokens_or_rows(handle):
     assert bool((dy == 0).all()) and bool((out == 0).all()) and bool((dw == 0).all())
 
 
-class Layer:
-    """A routed layer y = combine(route(x W_r), grouped(quantize(x[rows]), W)) and its gradients, on the calls."""
-
-    def __init__(self, h, gen, tokens, experts, top_k, d_in, d_out, align=128):
-        self.h, self.t, self.e, self.k, self.i, self.o, self.align = h, tokens, experts, top_k, d_in, d_out, align
-        self.w = (torch.randn(experts, d_out, d_in, generator=gen) * d_in ** -0.5).cuda()
-        self.rows = gs.moe_rows(tokens, experts, top_k, align)
-        i32 = dict(dtype=torch.int32, device="cuda")
-        self.ids, self.slot_row = torch.empty(tokens, top_k, **i32), torch.empty(tokens, top_k, **i32)
-        self.offsets, self.row_slot = torch.empty(experts + 1, **i32), torch.empty(self.rows, **i32)
-        self.p = torch.empty(tokens, top_k, device="cuda")
-        ws = gs.moe_route_workspace(tokens, experts, top_k)
-        self.ws, self.ws_bytes = torch.empty(max(ws, 4), dtype=torch.uint8, device="cuda"), ws
-        u8, f32, r = dict(dtype=torch.uint8, device="cuda"), dict(device="cuda"), self.rows
-        kb_i, kb_o, rb = blocks(d_in), blocks(d_out), blocks(r)
-        self.wq, self.ws_w = torch.empty(experts, d_out, d_in, **u8), torch.empty(experts, kb_o, kb_i, **f32)
-        self.xq, self.xs = torch.empty(r, d_in, **u8), torch.empty(kb_i, r, **f32)
-        self.xtq, self.xts = torch.empty(r, d_in, **u8), torch.empty(rb, d_in, **f32)
-        self.y = torch.zeros(r, d_out, dtype=torch.bfloat16, device="cuda")
-        self.out = torch.empty(tokens, d_out, dtype=torch.bfloat16, device="cuda")
-        self.dy = torch.empty_like(self.y)
-        self.dp, self.dlogits = torch.empty(tokens, top_k, **f32), torch.empty(tokens, experts, **f32)
-        self.gq, self.gs_ = torch.empty(r, d_out, **u8), torch.empty(kb_o, r, **f32)
-        self.gtq, self.gts = torch.empty(r, d_out, **u8), torch.empty(rb, d_out, **f32)
-        self.dx = torch.zeros(r, d_in, dtype=torch.bfloat16, device="cuda")
-        self.dx_tokens = torch.empty(tokens, d_in, dtype=torch.bfloat16, device="cuda")
-        self.dw = torch.empty(experts, d_out, d_in, **f32)
-
-    def cast_weights(self):
-        for e in range(self.e):
-            self.h.fp8_quantize(gs.SCALE_BLK128, 0, self.i, self.o, self.w[e], gs.R_32F, self.i, self.wq[e], gs.R_8F_E4M3, self.i,
-                                self.ws_w[e], blocks(self.i))
-
-    def forward(self, x, logits):
-        h, E4, VEC, BLK = self.h, gs.R_8F_E4M3, gs.SCALE_VEC128, gs.SCALE_BLK128
-        h.moe_route(self.t, self.e, self.k, logits, gs.R_32F, self.e, self.ids, self.p, renormalize=True, align=self.align,
-                    offsets=self.offsets, slot_row=self.slot_row, row_slot=self.row_slot, rows=self.rows, workspace=self.ws,
-                    workspace_bytes=self.ws_bytes)
-        h.fp8_quantize(VEC, 0, self.i, self.rows, x, gs.R_16BF, self.i, self.xq, E4, self.i, self.xs, self.rows,
-                       index=self.row_slot, index_div=self.k, src_cols=self.t)
-        h.gemm_fp8_grouped(gs.GROUP_N, gs.OP_T, gs.OP_N, self.o, self.rows, self.i, self.e, self.offsets, 1.0, self.wq, E4, self.i,
-                           self.o * self.i, self.ws_w, BLK, blocks(self.i), blocks(self.i) * blocks(self.o), self.xq, E4, self.i,
-                           self.xs, VEC, self.rows, 0.0, self.y, gs.R_16BF, self.o, 0)
-        h.moe_combine(self.t, self.k, self.o, self.y, gs.R_16BF, self.o, self.rows, self.slot_row, self.p, self.out, gs.R_16BF,
-                      self.o)
-
-    def backward(self, x, logits, dout):
-        h, E4, E5, VEC, BLK = self.h, gs.R_8F_E4M3, gs.R_8F_E5M2, gs.SCALE_VEC128, gs.SCALE_BLK128
-        h.moe_combine_backward(self.t, self.k, self.o, self.y, gs.R_16BF, self.o, self.rows, self.slot_row, self.row_slot, self.p,
-                               dout, gs.R_16BF, self.o, self.dy, self.o, self.dp)
-        h.moe_route_backward(self.t, self.e, self.k, logits, gs.R_32F, self.e, self.ids, self.dp, self.dlogits, gs.R_32F, self.e,
-                             renormalize=True)
-        h.fp8_quantize(VEC, 0, self.o, self.rows, self.dy, gs.R_16BF, self.o, self.gq, E5, self.o, self.gs_, self.rows)
-        h.fp8_quantize(VEC, 1, self.o, self.rows, self.dy, gs.R_16BF, self.o, self.gtq, E5, self.o, self.gts, self.o)
-        h.fp8_quantize(VEC, 1, self.i, self.rows, x, gs.R_16BF, self.i, self.xtq, E4, self.i, self.xts, self.i,
-                       index=self.row_slot, index_div=self.k, src_cols=self.t)
-        h.gemm_fp8_grouped(gs.GROUP_N, gs.OP_N, gs.OP_N, self.i, self.rows, self.o, self.e, self.offsets, 1.0, self.wq, E4, self.i,
-                           self.o * self.i, self.ws_w, BLK, blocks(self.i), blocks(self.i) * blocks(self.o), self.gq, E5, self.o,
-                           self.gs_, VEC, self.rows, 0.0, self.dx, gs.R_16BF, self.i, 0)
-        h.moe_combine(self.t, self.k, self.i, self.dx, gs.R_16BF, self.i, self.rows, self.slot_row, None, self.dx_tokens,
-                      gs.R_16BF, self.i)
-        h.gemm_fp8_grouped(gs.GROUP_K, gs.OP_N, gs.OP_T, self.i, self.o, self.rows, self.e, self.offsets, 1.0, self.xtq, E4, self.i,
-                           0, self.xts, VEC, self.i, 0, self.gtq, E5, self.o, self.gts, VEC, self.o, 0.0, self.dw, gs.R_32F, self.i,
-                           self.o * self.i)
-
-
-def reference_layer(layer, x, logits, dout):
+def reference_layer(layer, w, x, logits, dout):
     """The layer in float64 with the same choice, without any cast: values and gradients."""
-    xs, ls, ws = (v.double().clone().requires_grad_() for v in (x, logits, layer.w))
+    xs, ls, ws = (v.double().clone().requires_grad_() for v in (x, logits, w))
     p = weights_of(ls, layer.ids.long(), SOFTMAX, True, 1.0)
-    out = sum(p[:, j, None] * torch.einsum("ti,toi->to", xs, ws[layer.ids[:, j].long()]) for j in range(layer.k))
+    out = sum(p[:, j, None] * torch.einsum("ti,toi->to", xs, ws[layer.ids[:, j].long()]) for j in range(layer.top_k))
     (out * dout.double()).sum().backward()
     return out.detach(), xs.grad, ls.grad, ws.grad
 
@@ -432,42 +367,43 @@ def off(a, b):
     return float((a.double() - b).norm() / b.norm())
 
 
-def run_layer(h, tokens=200, experts=6, top_k=2, d_in=256, d_out=384):
-    gen = torch.Generator().manual_seed(21)
-    layer = Layer(h, gen, tokens, experts, top_k, d_in, d_out)
+def make_layer(h, tokens=200, experts=6, top_k=2, d_in=256, d_out=384, align=128, seed=21, **kw):
+    gen = torch.Generator().manual_seed(seed)
+    layer = RoutedExperts(h, tokens, experts, top_k, d_in, d_out, align, **kw)
+    w = (torch.randn(experts, d_out, d_in, generator=gen) * d_in ** -0.5).cuda()
+    layer.set_weights(w)
     x = torch.randn(tokens, d_in, generator=gen).to(torch.bfloat16).cuda()
     logits = torch.randn(tokens, experts, generator=gen).cuda()
     dout = torch.randn(tokens, d_out, generator=gen).to(torch.bfloat16).cuda()
-    return layer, x, logits, dout
+    return layer, w, x, logits, dout
 
 
-def check_layer(layer, x, logits, dout):
-    out, dx, dl, dw = reference_layer(layer, x, logits, dout)
+def check_layer(layer, w, x, logits, dout):
+    out, dx, dl, dw = reference_layer(layer, w, x, logits, dout)
+    b = layer._grad
     # Every product has two operands rounded to FP8: at most 2^-4 of a value each (E4M3), 2^-3 (E5M2), and independent
     # between terms, so the norm of a long sum is off by less than the two shares added; bf16 adds 2^-8 per store.
     assert off(layer.out, out) < 2 * 2.0 ** -4 + 2 * 2.0 ** -8
-    assert off(layer.dx_tokens, dx) < 2.0 ** -4 + 2.0 ** -3 + 3 * 2.0 ** -8
-    assert off(layer.dw, dw) < 2.0 ** -4 + 2.0 ** -3 + 2.0 ** -8
-    assert off(layer.dlogits, dl) < 2 * 2.0 ** -4 + 2 * 2.0 ** -8
+    assert off(b["dx"], dx) < 2.0 ** -4 + 2.0 ** -3 + 3 * 2.0 ** -8
+    assert off(b["dw"], dw) < 2.0 ** -4 + 2.0 ** -3 + 2.0 ** -8
+    assert off(b["dlogits"], dl) < 2 * 2.0 ** -4 + 2 * 2.0 ** -8
 
 
 def test_a_routed_layer_and_its_gradients(handle):
-    layer, x, logits, dout = run_layer(handle)
-    layer.cast_weights()
+    layer, w, x, logits, dout = make_layer(handle)
     layer.forward(x, logits)
     layer.backward(x, logits, dout)
     torch.cuda.synchronize()
     assert handle.device_error() == 0
-    check_layer(layer, x, logits, dout)
+    check_layer(layer, w, x, logits, dout)
 
 
 def test_a_routed_layer_captured_and_replayed_on_new_inputs(cuda):
     stream = torch.cuda.Stream()
     with gs.Handle(stream) as h:
-        layer, x, logits, dout = run_layer(h, tokens=700)
         torch.cuda.synchronize()
         with torch.cuda.stream(stream):
-            layer.cast_weights()
+            layer, w, x, logits, dout = make_layer(h, tokens=700)
             layer.forward(x, logits)
             layer.backward(x, logits, dout)
         stream.synchronize()
@@ -482,18 +418,58 @@ def test_a_routed_layer_captured_and_replayed_on_new_inputs(cuda):
             g.replay()
         torch.cuda.synchronize()
         assert h.device_error() == 0
-        check_layer(layer, x, logits, dout)
+        check_layer(layer, w, x, logits, dout)
         del g
 
 
 @pytest.mark.parametrize("tokens", [1, 3])
 def test_a_routed_layer_for_single_tokens(handle, tokens):
-    gen = torch.Generator().manual_seed(tokens)
-    layer = Layer(handle, gen, tokens, 16, 4, 512, 256, align=1)
-    layer.cast_weights()
-    x = torch.randn(tokens, 512, generator=gen).to(torch.bfloat16).cuda()
-    logits = torch.randn(tokens, 16, generator=gen).cuda()
+    layer, w, x, logits, dout = make_layer(handle, tokens, 16, 4, 512, 256, align=1, seed=tokens)
     layer.forward(x, logits)
     torch.cuda.synchronize()
-    out, _, _, _ = reference_layer(layer, x, logits, torch.ones(tokens, 256, device="cuda"))
+    out, _, _, _ = reference_layer(layer, w, x, logits, dout)
     assert off(layer.out, out) < 2 * 2.0 ** -4 + 2 * 2.0 ** -8
+    with pytest.raises(ValueError):
+        layer.backward(x, logits, dout)  # its plan is not aligned
+
+
+def test_a_routed_layer_with_a_padded_batch(handle):
+    """Tokens past token_count (padding of a captured batch, here NaN) reach no expert and leave no trace in the others."""
+    count = torch.tensor([150], dtype=torch.int32, device="cuda")
+    layer, w, x, logits, dout = make_layer(handle, token_count=count)
+    x[150:], logits[150:], dout[150:] = math.nan, math.nan, 0.0
+    layer.forward(x, logits)
+    layer.backward(x, logits, dout)
+    torch.cuda.synchronize()
+    assert bool((layer.out[150:] == 0).all()) and bool((layer._grad["dx"][150:] == 0).all())
+    out, dx, _, dw = reference_layer_of(layer, w, x[:150], logits[:150], dout[:150])
+    assert off(layer.out[:150], out) < 2 * 2.0 ** -4 + 2 * 2.0 ** -8
+    assert off(layer._grad["dx"][:150], dx) < 2.0 ** -4 + 2.0 ** -3 + 3 * 2.0 ** -8
+    assert off(layer._grad["dw"], dw) < 2.0 ** -4 + 2.0 ** -3 + 2.0 ** -8
+
+
+def reference_layer_of(layer, w, x, logits, dout):
+    class Part:
+        ids, top_k = layer.ids[:x.shape[0]], layer.top_k
+
+    return reference_layer(Part, w, x, logits, dout)
+
+
+def test_two_layers_on_two_streams_at_once(cuda):
+    """An instance and a handle to each stream, sharing the weight blocks."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    with gs.Handle(streams[0]) as h0, gs.Handle(streams[1]) as h1:
+        with torch.cuda.stream(streams[0]):
+            layer, w, x, logits, dout = make_layer(h0, tokens=900)
+        torch.cuda.synchronize()
+        other = RoutedExperts(h1, 900, 6, 2, 256, 384, weights_of=layer)
+        for _ in range(3):
+            for l, s in ((layer, streams[0]), (other, streams[1])):
+                with torch.cuda.stream(s):
+                    l.forward(x, logits)
+                    l.backward(x, logits, dout)
+        torch.cuda.synchronize()
+        check_layer(layer, w, x, logits, dout)
+        for name in ("dx", "dlogits", "dw"):
+            assert torch.equal(layer._grad[name], other._grad[name])
+        assert torch.equal(layer.out, other.out)
