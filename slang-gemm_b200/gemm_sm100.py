@@ -9,7 +9,8 @@ CUDA tensors. `host_gemm_ex` mirrors `gemm.gemmEx` (src/gemm.zig:546) over
 host numpy buffers.
 
 There is no CPU fallback: importing this module fails if the shared library
-has not been built, and every call fails without an sm_100 device.
+(and `_gs_fastcall`, the native binding of the FP8 and routed-expert calls) has
+not been built, and every call fails without an sm_100 device.
 """
 from __future__ import annotations
 
@@ -198,6 +199,8 @@ def _load() -> ctypes.CDLL:
 
 _lib = _load()
 
+import _gs_fastcall as _fast  # noqa: E402  (needs the library; built beside it by the same make)
+
 
 def lib() -> ctypes.CDLL:
     return _lib
@@ -333,13 +336,14 @@ class Handle:
         if s != STATUS_SUCCESS:
             raise GemmError(s, "gs_create")
         self._h = h
+        self._raw = h.value  # the address, for _gs_fastcall
         if stream is not None:
             self.set_stream(stream)
 
     def close(self):
         if self._h:
             _lib.gs_destroy(self._h)
-            self._h = None
+            self._h = self._raw = None
 
     def __enter__(self):
         return self
@@ -356,8 +360,7 @@ class Handle:
     # ---- handle state ----
     def set_stream(self, stream):
         """stream: a torch.cuda.Stream, a raw cudaStream_t int, or None."""
-        ptr = getattr(stream, "cuda_stream", stream)
-        self._check(_lib.gs_set_stream(self._h, ptr), "gs_set_stream")
+        self._check(_fast.set_stream(self._raw, getattr(stream, "cuda_stream", stream)), "gs_set_stream")
 
     def last_error(self) -> str:
         return _lib.gs_last_error(self._h).decode()
@@ -445,18 +448,16 @@ class Handle:
     def fp8_quantize(self, mode, axis, rows, cols, src, src_type, ld_src, dst, dst_type, ld_dst, scale, ld_scale,
                      index=None, index_div=1, src_cols=0, check=True) -> int:
         """Column-major rows x cols `src` to FP8 `dst` with power-of-two scales; see gs_fp8_quantize."""
-        s = _lib.gs_fp8_quantize(self._h, mode, axis, rows, cols, _ptr(src), src_type, ld_src, _ptr(index), index_div,
-                                 src_cols, _ptr(dst), dst_type, ld_dst, _ptr(scale), ld_scale)
+        s = _fast.fp8_quantize(self._raw, mode, axis, rows, cols, src, src_type, ld_src, index, index_div, src_cols, dst,
+                               dst_type, ld_dst, scale, ld_scale)
         if check:
             self._check(s, "gs_fp8_quantize")
         return s
 
     def gemm_fp8(self, transa, transb, m, n, k, alpha, A, atype, lda, a_scale, a_mode, ldsa, B, btype, ldb, b_scale,
                  b_mode, ldsb, beta, C, ctype, ldc, check=True) -> int:
-        a, b = ctypes.c_float(alpha), ctypes.c_float(beta)
-        s = _lib.gs_gemm_fp8(self._h, transa, transb, m, n, k, ctypes.byref(a), _ptr(A), atype, lda, _ptr(a_scale),
-                             a_mode, ldsa, _ptr(B), btype, ldb, _ptr(b_scale), b_mode, ldsb, ctypes.byref(b), _ptr(C),
-                             ctype, ldc)
+        s = _fast.gemm_fp8(self._raw, transa, transb, m, n, k, alpha, A, atype, lda, a_scale, a_mode, ldsa, B, btype, ldb,
+                           b_scale, b_mode, ldsb, beta, C, ctype, ldc)
         if check:
             self._check(s, "gs_gemm_fp8")
         return s
@@ -465,11 +466,9 @@ class Handle:
                          a_mode, ldsa, stride_sa, B, btype, ldb, b_scale, b_mode, ldsb, beta, C, ctype, ldc, stride_c,
                          check=True) -> int:
         """offsets: groups + 1 int32 device values along the ragged axis (GROUP_N: columns of B and C; GROUP_K: K)."""
-        a, b = ctypes.c_float(alpha), ctypes.c_float(beta)
-        s = _lib.gs_gemm_fp8_grouped(self._h, ragged, transa, transb, m, n, k, groups, _ptr(offsets), ctypes.byref(a),
-                                     _ptr(A), atype, lda, stride_a, _ptr(a_scale), a_mode, ldsa, stride_sa, _ptr(B),
-                                     btype, ldb, _ptr(b_scale), b_mode, ldsb, ctypes.byref(b), _ptr(C), ctype, ldc,
-                                     stride_c)
+        s = _fast.gemm_fp8_grouped(self._raw, ragged, transa, transb, m, n, k, groups, offsets, alpha, A, atype, lda,
+                                   stride_a, a_scale, a_mode, ldsa, stride_sa, B, btype, ldb, b_scale, b_mode, ldsb, beta,
+                                   C, ctype, ldc, stride_c)
         if check:
             self._check(s, "gs_gemm_fp8_grouped")
         return s
@@ -479,10 +478,9 @@ class Handle:
                   offsets=None, slot_row=None, row_slot=None, rows=0, workspace=None, workspace_bytes=0,
                   check=True) -> int:
         """Expert choice and weights, and with `offsets` the row plan of the grouped products; see gs_moe_route."""
-        d = RouteDesc(tokens, experts, top_k, _ptr(logits), logits_type, ld_logits, _ptr(bias), score, groups,
-                      top_groups, int(renormalize), scale, _ptr(token_count), align, _ptr(ids), _ptr(weights),
-                      _ptr(offsets), _ptr(slot_row), _ptr(row_slot), rows, _ptr(workspace), workspace_bytes)
-        s = _lib.gs_moe_route(self._h, ctypes.byref(d))
+        s = _fast.moe_route(self._raw, tokens, experts, top_k, logits, logits_type, ld_logits, bias, score, groups,
+                            top_groups, renormalize, scale, token_count, align, ids, weights, offsets, slot_row, row_slot,
+                            rows, workspace, workspace_bytes)
         if check:
             self._check(s, "gs_moe_route")
         return s
@@ -490,17 +488,17 @@ class Handle:
     def moe_route_backward(self, tokens, experts, top_k, logits, logits_type, ld_logits, ids, dweights, dlogits,
                            dlogits_type, ld_dlogits, score=ROUTE_SOFTMAX, renormalize=False, scale=1.0,
                            check=True) -> int:
-        d = RouteDesc(tokens=tokens, experts=experts, top_k=top_k, logits=_ptr(logits), logits_type=logits_type,
-                      ld_logits=ld_logits, score=score, renormalize=int(renormalize), scale=scale, ids=_ptr(ids))
-        s = _lib.gs_moe_route_backward(self._h, ctypes.byref(d), _ptr(dweights), _ptr(dlogits), dlogits_type, ld_dlogits)
+        s = _fast.moe_route_backward(self._raw, tokens, experts, top_k, logits, logits_type, ld_logits, None, score, 1, 1,
+                                     renormalize, scale, None, 1, ids, None, None, None, None, 0, None, 0, dweights,
+                                     dlogits, dlogits_type, ld_dlogits)
         if check:
             self._check(s, "gs_moe_route_backward")
         return s
 
     def moe_combine(self, tokens, top_k, hidden, y, ytype, ldy, rows, slot_row, weights, out, out_type, ld_out,
                     check=True) -> int:
-        s = _lib.gs_moe_combine(self._h, tokens, top_k, hidden, _ptr(y), ytype, ldy, rows, _ptr(slot_row),
-                                _ptr(weights), _ptr(out), out_type, ld_out)
+        s = _fast.moe_combine(self._raw, tokens, top_k, hidden, y, ytype, ldy, rows, slot_row, weights, out, out_type,
+                              ld_out)
         if check:
             self._check(s, "gs_moe_combine")
         return s
@@ -510,9 +508,8 @@ class Handle:
         """dout and dy have y's type (dout_type must be ytype)."""
         if dout_type != ytype:
             raise ValueError("dout must have y's type")
-        s = _lib.gs_moe_combine_backward(self._h, tokens, top_k, hidden, _ptr(y), ytype, ldy, rows, _ptr(slot_row),
-                                         _ptr(row_slot), _ptr(weights), _ptr(dout), ld_dout, _ptr(dy), ld_dy,
-                                         _ptr(dweights))
+        s = _fast.moe_combine_backward(self._raw, tokens, top_k, hidden, y, ytype, ldy, rows, slot_row, row_slot, weights,
+                                       dout, ld_dout, dy, ld_dy, dweights)
         if check:
             self._check(s, "gs_moe_combine_backward")
         return s

@@ -178,3 +178,51 @@ def test_plan_tile():
     assert gs.plan_gemm_fp8(1, 0, 2048, 128, 2048, groups=64)[1:] == (32, 1, 1)
     for bad in (dict(m=0, n=1, k=1), dict(m=1, n=1, k=1, groups=gs.FP8_MAX_GROUPS + 1), dict(m=1, n=1, k=1, groups=1, ragged=5)):
         assert gs.plan_gemm_fp8(1, 0, **bad)[0] == gs.STATUS_INVALID_VALUE
+
+
+class Pointer:
+    """Stands for a tensor: something with a data_ptr()."""
+
+    def __init__(self, at):
+        self.at = at
+
+    def data_ptr(self):
+        return self.at
+
+
+def test_native_binding_passes_arguments_through():
+    """_gs_fastcall hands the library the same arguments as ctypes does: the statuses agree, whatever kind of pointer."""
+    import _gs_fastcall as fast
+
+    def call(p, m=256, lda=512, ldb=512, at=gs.R_8F_E4M3):
+        return fast.gemm_fp8(None, 1, 0, m, 96, 512, 1.0, p, at, lda, p, gs.SCALE_BLK128, 4, p, gs.R_8F_E5M2, ldb, p,
+                             gs.SCALE_VEC128, 96, 0, p, gs.R_16BF, 256)
+
+    for p in (P, Pointer(P)):
+        assert call(p) == OK
+        assert call(p, lda=496) == BAD and call(p, at=gs.R_8I) == UNS
+    assert call(None) == BAD and call(P + 8) == UNS and call(P, m=0) == OK
+    assert fast.fp8_quantize(None, gs.SCALE_VEC128, 0, 256, 128, P, gs.R_16BF, 256, None, 1, 0, P, gs.R_8F_E4M3, 256, P,
+                             127) == BAD
+    assert fast.moe_combine(None, 8, 2, 64, P, gs.R_16BF, 64, 16, P, None, P, gs.R_16BF, 64) == OK
+    route = [2048, 64, 4, P, gs.R_32F, 64, None, gs.ROUTE_SIGMOID, 8, 2, True, 2.5, None, 128, P, P, P, P, P, 2**16, P, 2**20]
+    assert fast.moe_route(None, *route) == OK
+    for k, v, status in ((2, 65, BAD), (5, 63, BAD), (9, 9, BAD), (13, 0, BAD), (19, 8192, BAD), (21, 16, BAD), (4, gs.R_8I, UNS)):
+        assert fast.moe_route(None, *route[:k], v, *route[k + 1:]) == status, k
+    assert fast.moe_route_backward(None, *route, P, P, gs.R_32F, 64) == OK
+    assert fast.moe_route_backward(None, *route, P, P, gs.R_32F, 63) == BAD
+    assert fast.moe_combine_backward(None, 8, 2, 64, P, gs.R_16BF, 64, 16, P, P, P, P, 64, P, 63, P) == BAD
+    assert fast.set_stream(None, None) == OK
+
+
+def test_native_binding_refuses_what_c_cannot_hold():
+    import _gs_fastcall as fast
+
+    with pytest.raises(TypeError):
+        fast.set_stream(None)
+    with pytest.raises(OverflowError):
+        fast.moe_combine(None, 2**31, 2, 64, P, gs.R_16BF, 64, 16, P, None, P, gs.R_16BF, 64)
+    with pytest.raises(TypeError):
+        fast.moe_combine(None, 1.5, 2, 64, P, gs.R_16BF, 64, 16, P, None, P, gs.R_16BF, 64)
+    with pytest.raises(AttributeError):
+        fast.moe_combine(None, 8, 2, 64, "y", gs.R_16BF, 64, 16, P, None, P, gs.R_16BF, 64)
