@@ -299,7 +299,8 @@ enum { GS_SCALE_VEC128 = 4, GS_SCALE_BLK128 = 5 }; /* cublasLtMatmulMatrixScale_
  * index: NULL, or cols int32 device values: column c is then read from source
  * column index[c] / indexDiv of srcCols; a negative index, or one past the
  * end, gives a column of zeros. With gs_moe_route's row_slot and indexDiv =
- * top_k the cast puts the tokens in expert order. src and dst must not overlap. */
+ * top_k the cast puts the tokens in expert order. src and dst must not overlap.
+ * rows and cols are at most 2^30. */
 gs_status gs_fp8_quantize(gs_handle handle, int scaleMode, int axis, int rows, int cols, const void *src, int srcType,
                           int ldsrc, const int32_t *index, int indexDiv, int srcCols, void *dst, int dstType, int lddst,
                           float *scale, int ldscale);
@@ -408,7 +409,8 @@ gs_status gs_moe_route_backward(gs_handle handle, const gs_route_desc *desc, con
 /* out[t] = sum over j of weights[t, j] * y[slot_row[t, j]] in f32, in the order
  * of j, rounded once; slots with row -1 (or outside [0, rows)) add nothing.
  * Rows of y and out are hidden elements at y + r*ldy, out + t*ldout. weights
- * NULL = 1, which makes it the gradient of the gather gs_fp8_quantize does. */
+ * NULL = 1, which makes it the gradient of the gather gs_fp8_quantize does.
+ * hidden is at most 2^30. */
 gs_status gs_moe_combine(gs_handle handle, int tokens, int top_k, int hidden, const void *y, int yType, int ldy,
                          int rows, const int32_t *slot_row, const float *weights, void *out, int outType, int ldout);
 

@@ -11,6 +11,7 @@ namespace gs {
 namespace {
 
 constexpr int kMaxDim = 0x7fffffff - 1024;  // 32-bit coordinates run up to one tile past the end
+constexpr int kMaxRow = 1 << 30;            // the element-wise kernels' run up to one block's step past it
 
 class DeviceGuard {
 public:
@@ -193,7 +194,7 @@ gs_status gs_fp8_quantize(gs_handle h, int mode, int axis, int rows, int cols, c
             if (index && (index_div < 1 || src_cols < 0)) return invalid("indexDiv must be positive and srcCols not negative");
             if (!float_type(src_type)) return unsupported("src must be R_32F, R_16F or R_16BF");
             if (!fp8_type(dst_type)) return unsupported("dst must be R_8F_E4M3 or R_8F_E5M2");
-            if (rows > kMaxDim || cols > kMaxDim) return unsupported("rows and cols are limited to 2^31 - 1025");
+            if (rows > kMaxRow || cols > kMaxRow) return unsupported("rows and cols are limited to 2^30");
             if (rows == 0 || cols == 0) {
                 *empty = true;
                 return {};
@@ -380,7 +381,7 @@ static Refusal check_combine(int tokens, int top_k, int hidden, const void *y, i
     if (top_k < 1) return invalid("top_k must be positive");
     if (ldy < at_least_1(hidden)) return invalid("ldy too small");
     if (!float_type(type)) return unsupported("y must be R_32F, R_16F or R_16BF");
-    if (static_cast<long long>(tokens) * top_k > kMaxDim || rows > kMaxDim || hidden > kMaxDim) return unsupported("too many slots or rows");
+    if (static_cast<long long>(tokens) * top_k > kMaxDim || rows > kMaxDim || hidden > kMaxRow) return unsupported("too many slots or rows, or hidden above 2^30");
     if (tokens > 0 && hidden > 0 && rows > 0 && !y) return invalid("y is null");
     if (tokens > 0 && !slot_row) return invalid("slot_row is null");
     if (!on(y, float_size(type)) || !on(slot_row, 4)) return invalid("misaligned pointer");

@@ -32,8 +32,9 @@
 //    cp.async, which completes on the ring's mbarriers;
 //  - warps 4..: promoters, BN / (warps / 4) columns each. With 128 columns a
 //    thread they need more registers than an even split gives: of the 3 x 168 a
-//    lane triple is launched with, the first warpgroup hands 96 to the two
-//    promoter warpgroups (72 / 216 / 216).
+//    lane triple is launched with, the first warpgroup hands 96 or 112 to the
+//    two promoter warpgroups (72 / 216 / 216, or 56 / 224 / 224 where the
+//    scale warp copies no vector of Q).
 // Ragged groups: offsets are read from device memory; tile counts are scanned
 // once per CTA into shared memory and each tile finds its group by bisection.
 //
@@ -260,15 +261,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     return v;
 }
 
-// Each thread of the warp reads 16 consecutive 32-bit columns of its TMEM lane.
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
 // Waits for two barriers, both polled once before either is waited for: a poll's latency is paid once.
 __device__ __forceinline__ bool mbar_wait2(uint64_t *b1, uint32_t parity1, uint32_t site1, uint64_t *b2, uint32_t parity2,
                                            uint32_t site2, uint32_t *err, long long limit) {
@@ -476,7 +468,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     Item it;
 
     if (warp < 4) {
-    if constexpr (EPI_COLS == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (EPI_COLS == 128) {
+        if constexpr (Q_VEC) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    }
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
@@ -598,7 +593,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
     }
     } else {
         // ---------------- promoters ----------------
-        if constexpr (EPI_COLS == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if constexpr (EPI_COLS == 128) {
+            if constexpr (Q_VEC) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+            else asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        }
         const int quad = warp & 3;
         const int ew = warp - 4;
         const int c_lo = (ew / 4) * EPI_COLS;
@@ -625,22 +623,22 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                     break;
                 }
                 tc_fence_after();
-                // The next 16 columns are on their way while these are added. (32 at a time spilled the sums: 0.67 instead
-                // of 0.58 us a K block.)
+                // The next 32 columns are on their way while these are added (16 at a time: 849 instead of 774 cycles a K
+                // block of a wide tile).
                 const uint32_t t_slot = t_lane + slot * BN + c_lo;
-                uint32_t r[2][16];
-                tmem_ld_x16(t_slot, r[0]);
+                uint32_t r[2][32];
+                tmem_ld_32x32b_x32(t_slot, r[0]);
                 const float *sc = scales + ss * C_::SC_FLOATS;
                 const uint32_t sc_addr = smem_u32(sc + c_lo);
                 float s = sc[BN + (P_VEC ? row : 0)];
                 if constexpr (!Q_VEC) s = __fmul_rn(s, sc[c_lo / 128]);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
-                for (int c = 0; c < EPI_COLS; c += 16) {
-                    const int cur = (c / 16) & 1;
+                for (int c = 0; c < EPI_COLS; c += 32) {
+                    const int cur = (c / 32) & 1;
                     tmem_wait_ld();
-                    if (c + 16 < EPI_COLS) {
-                        tmem_ld_x16(t_slot + c + 16, r[cur ^ 1]);
+                    if (c + 32 < EPI_COLS) {
+                        tmem_ld_32x32b_x32(t_slot + c + 32, r[cur ^ 1]);
                     } else {  // the slot is read: the tensor core may fill it again
                         tc_fence_before();
                         __syncwarp();
@@ -650,7 +648,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
+                    for (int j = 0; j < 32; j += 4) {
                         const uint64_t p0 = pack2(__uint_as_float(r[cur][j]), __uint_as_float(r[cur][j + 1]));
                         const uint64_t p1 = pack2(__uint_as_float(r[cur][j + 2]), __uint_as_float(r[cur][j + 3]));
                         uint64_t &a0 = acc[(c + j) / 2], &a1 = acc[(c + j) / 2 + 1];
@@ -888,7 +886,7 @@ static bool aligned_c(const GemmFp8Desc &d) {
 
 // Tile of a product: bn columns, cg CTAs, split K slices. Each kind of tile is given the microseconds that its K blocks
 // and the rest of it took in a sweep of 13 shapes from 512^3 to 8192^3, dense and ragged, alone on the GPU (a pair's 256 x 256
-// tile 0.50 a K block, 0.86 with a scale per row and per column; 128 x 128, 64 and 32 tiles of one SM 0.41, 0.30 and
+// tile 0.46 a K block, 0.82 with a scale per row and per column; 128 x 128, 64 and 32 tiles of one SM 0.41, 0.30 and
 // 0.25); the cheapest rounds-times-tile wins. Against a rule on the column count alone: 1024^3 12.5 -> 6.9 us, 1024 x 1024 x 4096
 // with both scales per vector 32 -> 17 us, 64 groups of 32 rows 82 -> 53 us.
 // Narrow tiles that leave SMs without work may share their K blocks over a cluster, as long as all clusters run at once
@@ -902,7 +900,7 @@ Tile choose_tile(const GemmFp8Desc &d, int sm_count) {
     const Kind kinds[4] = {{32, 0.25, 1.1, 0.5},
                            {64, 0.30, 1.25, 0.5},
                            {128, 0.41, 1.7, 0.5},
-                           {256, d.a_vec ? (d.b_vec ? 0.86 : 0.75) : 0.50, !aligned_c(d) ? 20.0 : f32_out ? 4.0 : 2.0, 0.75}};
+                           {256, d.a_vec ? (d.b_vec ? 0.82 : 0.72) : 0.46, !aligned_c(d) ? 20.0 : f32_out ? 4.0 : 2.0, 0.75}};
     Tile best{2, 256, 1};
     double least = 1e300;
     for (const Kind &kind : kinds) {

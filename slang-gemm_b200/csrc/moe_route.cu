@@ -607,6 +607,9 @@ __global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ 
     const int lane = threadIdx.x & 31;
     for (long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < d.tokens; t += static_cast<long long>(gridDim.x) * 8) {
         const T *logits = static_cast<const T *>(d.logits) + t * d.ld;
+        const bool every = !d.renorm && !d.sigmoid;  // softmax that is not renormalised: every logit has a gradient
+        float l[VPL];
+        if (every) load_row<T, VPL>(logits, d.experts, lane, l);  // on its way while the ids come in
         int id = -1;
         float g = 0.0f, x = -INFINITY;  // lane j: the j-th chosen expert, its weight's gradient and its logit
         if (lane < d.top_k) {
@@ -638,8 +641,6 @@ __global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ 
         } else if (d.sigmoid) {
             slope = g / (1.0f + expf(-x)) * (1.0f / (1.0f + expf(x)));
         } else {
-            float l[VPL];
-            load_row<T, VPL>(logits, d.experts, lane, l);
             const float top = row_top(l);
             float sum = 0.0f;
 #pragma unroll
@@ -656,7 +657,6 @@ __global__ void __launch_bounds__(256) k_route_backward(const __grid_constant__ 
         }
         if (id < 0) slope = 0.0f;
         float out[VPL];
-        const bool every = !d.renorm && !d.sigmoid;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) out[i] = every ? -common * s[i] : 0.0f;
         for (int j = 0; j < d.top_k; ++j) {
@@ -702,7 +702,7 @@ cudaError_t launch_route(Context &ctx, const RouteDesc &d) {
 
 cudaError_t launch_route_backward(Context &ctx, const RouteBwdDesc &d) {
     ctx.last_kernels |= GS_KERNEL_ROUTE;
-    const long long want = (static_cast<long long>(d.tokens) + 7) / 8, most = 8LL * ctx.sm_count;
+    const long long want = (static_cast<long long>(d.tokens) + 7) / 8, most = 32LL * ctx.sm_count;
     const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
     return with_float_type(d.type, [&](auto z) {
         return route::with_vpl(d.experts, [&](auto v) {

@@ -30,7 +30,8 @@ def quantize(mode=gs.SCALE_VEC128, axis=0, rows=256, cols=128, src=P, st=gs.R_16
     ({"mode": gs.SCALE_BLK128, "ldsc": 1}, BAD), ({"index": P, "div": 0}, BAD), ({"index": P, "src_cols": -1}, BAD),
     ({"src": None}, BAD), ({"dst": None}, BAD), ({"scale": None}, BAD), ({"src": P + 1}, BAD), ({"scale": P + 2}, BAD),
     ({"index": P + 1, "src_cols": 4}, BAD), ({"st": gs.R_8I}, UNS), ({"dt": gs.R_16F}, UNS),
-    ({"cols": 2**31 - 1, "ldsc": 2**31 - 1}, UNS),
+    ({"cols": 2**31 - 1, "ldsc": 2**31 - 1}, UNS), ({"rows": 2**30 + 1, "lds": 2**31 - 1, "ldd": 2**31 - 1}, UNS),
+    ({"rows": 2**30, "lds": 2**30, "ldd": 2**30}, OK),
 ])
 def test_quantize_checks(change, status):
     assert quantize(**change) == status
@@ -131,6 +132,7 @@ def combine(tokens=8, top_k=2, hidden=64, y=P, yt=gs.R_16BF, ldy=64, rows=16, sl
     ({"tokens": -1}, BAD), ({"top_k": 0}, BAD), ({"hidden": -1}, BAD), ({"ldy": 63}, BAD), ({"ldo": 63}, BAD), ({"y": None}, BAD),
     ({"slot": None}, BAD), ({"out": None}, BAD), ({"y": P + 1}, BAD), ({"w": P + 2}, BAD), ({"out": P + 1}, BAD),
     ({"yt": gs.R_8I}, UNS), ({"ot": gs.R_8F_E4M3}, UNS), ({"tokens": 2**30, "top_k": 4}, UNS),
+    ({"hidden": 2**30 + 1, "ldy": 2**31 - 1, "ldo": 2**31 - 1}, UNS),
 ])
 def test_combine_checks(change, status):
     assert combine(**change) == status
