@@ -55,11 +55,11 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     const uint32_t lo = __reduce_max_sync(kFull, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
-// Fast forms for the choice, whose f32 errors it allows for, and accurate ones.
-template <bool FAST> __device__ __forceinline__ float exp_of(float x) { return FAST ? __expf(x) : expf(x); }
-template <bool FAST> __device__ __forceinline__ double exp_of(double x) { return exp(x); }
-template <bool FAST> __device__ __forceinline__ float inverse(float x) { return FAST ? __fdividef(1.0f, x) : 1.0f / x; }
-template <bool FAST> __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
+// The choice's exponential and reciprocal: fast in f32, whose errors `doubt` allows for.
+__device__ __forceinline__ float exp_of(float x) { return __expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float inverse(float x) { return __fdividef(1.0f, x); }
+__device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
 template <typename R>
 __device__ __forceinline__ R warp_sum(R v) {
 #pragma unroll
@@ -89,17 +89,21 @@ __device__ __forceinline__ float row_top(const float (&l)[VPL]) {
     return value_of(warp_max(key_of(top)));
 }
 // Scores of all experts (masked ones: 0). top: softmax's largest logit.
-template <bool FAST, typename R, int VPL>
+template <typename R, int VPL>
 __device__ __forceinline__ void scores(const float (&l)[VPL], bool sigmoid, float top, R (&s)[VPL]) {
     if (sigmoid) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) s[i] = l[i] == -INFINITY ? R(0) : inverse<FAST>(R(1) + exp_of<FAST>(-R(fmaxf(l[i], FAST ? -80.0f : l[i]))));
+        for (int i = 0; i < VPL; ++i) {
+            // f32: below -80 a sigmoid is 0 to within the doubt, and the fast quotient's range ends
+            const R x = std::is_same<R, float>::value ? R(fmaxf(l[i], -80.0f)) : R(l[i]);
+            s[i] = l[i] == -INFINITY ? R(0) : inverse(R(1) + exp_of(-x));
+        }
         return;
     }
     R sum = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-        s[i] = l[i] == -INFINITY ? R(0) : exp_of<FAST>(R(l[i]) - R(top));
+        s[i] = l[i] == -INFINITY ? R(0) : exp_of(R(l[i]) - R(top));
         sum += s[i];
     }
     sum = warp_sum(sum);
@@ -145,7 +149,7 @@ __device__ __forceinline__ bool choose_sorted(const RouteDesc &d, const uint32_t
         }
     }
     uint32_t least = __shfl_sync(kFull, m, d.top_k - 1);
-    if (d.bias != nullptr && least > none) {
+    if (d.bias != nullptr && least > none && value_of(least) < INFINITY) {
         const float v = value_of(least);
         least = key_of(v - 2.0f * doubt(d, v));
     }
@@ -226,7 +230,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
     auto far = [&](float x, float y, float terms) { return !(fabsf(x - y) <= 2.0f * terms * doubt(d, x)); };
     if (d.bias != nullptr || grouped) {
         R s[VPL];
-        scores<F32, R, VPL>(l, d.sigmoid != 0, top, s);
+        scores<R, VPL>(l, d.sigmoid != 0, top, s);
         Key ck[VPL];  // by c, which is what groups compare
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
@@ -545,21 +549,41 @@ __global__ void __launch_bounds__(kPlanThreads) k_route_plan(const __grid_consta
     const int ahead = a + static_cast<int>(threadIdx.x & 31) < b ? d.ids[a + (threadIdx.x & 31)] : -1;  // while the counts come in
     for (int i = threadIdx.x; i < 2 * experts; i += kPlanThreads) sm[i] = 0;
     __syncthreads();
-    const int parts = max(1, kPlanThreads / experts), blocks = gridDim.x;
-    for (int i = threadIdx.x; i < experts * parts; i += kPlanThreads) {
-        const int e = i % experts, part = i / experts;
-        int all = 0, mine = 0;
-        // Each block begins at its own row, so that they do not all read the same lines at once.
+    // Each block begins at its own row, so that they do not all read the same lines at once.
+    const int blocks = gridDim.x, self = static_cast<int>(blockIdx.x);
+    if (experts % 4 == 0 && reinterpret_cast<uintptr_t>(d.hist) % 16 == 0) {  // four experts to a thread
+        const int quads = experts / 4, parts = kPlanThreads / quads;  // experts <= 1024
+        const int e = threadIdx.x % quads, part = threadIdx.x / quads;
+        if (part < parts) {
+            int4 all = make_int4(0, 0, 0, 0), mine = make_int4(0, 0, 0, 0);
+            const int4 *hist = reinterpret_cast<const int4 *>(d.hist) + e;
 #pragma unroll 8
-        for (int x = part; x < blocks; x += parts) {
-            int b = x + static_cast<int>(blockIdx.x);
-            if (b >= blocks) b -= blocks;
-            const int n = d.hist[static_cast<long long>(b) * experts + e];
-            all += n;
-            if (b < static_cast<int>(blockIdx.x)) mine += n;
+            for (int x = part; x < blocks; x += parts) {
+                const int b = x + self < blocks ? x + self : x + self - blocks;
+                const int4 n = hist[b * quads];  // at most 148 x 256
+                all.x += n.x; all.y += n.y; all.z += n.z; all.w += n.w;
+                if (b < self) { mine.x += n.x; mine.y += n.y; mine.z += n.z; mine.w += n.w; }
+            }
+            atomicAdd(&count[4 * e], all.x); atomicAdd(&count[4 * e + 1], all.y);
+            atomicAdd(&count[4 * e + 2], all.z); atomicAdd(&count[4 * e + 3], all.w);
+            atomicAdd(&before[4 * e], mine.x); atomicAdd(&before[4 * e + 1], mine.y);
+            atomicAdd(&before[4 * e + 2], mine.z); atomicAdd(&before[4 * e + 3], mine.w);
         }
-        atomicAdd(&count[e], all);
-        atomicAdd(&before[e], mine);
+    } else {
+        const int parts = max(1, kPlanThreads / experts);
+        for (int i = threadIdx.x; i < experts * parts; i += kPlanThreads) {
+            const int e = i % experts, part = i / experts;
+            int all = 0, mine = 0;
+#pragma unroll 8
+            for (int x = part; x < blocks; x += parts) {
+                const int b = x + self < blocks ? x + self : x + self - blocks;
+                const int n = d.hist[b * experts + e];
+                all += n;
+                if (b < self) mine += n;
+            }
+            atomicAdd(&count[e], all);
+            atomicAdd(&before[e], mine);
+        }
     }
     __syncthreads();
     expert_bases<kPlanThreads>(count, base, experts, d.align);

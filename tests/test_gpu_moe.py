@@ -115,6 +115,8 @@ def check_route(got, logits, k, score, bias, groups, top_groups, renorm, scale, 
     (70, 1024, 32, SOFTMAX, False, 32, 4, False, 1.0, 4, torch.float32),
     (2000, 8, 2, SOFTMAX, False, 1, 1, True, 1.0, 128, torch.float16),
     (700, 6, 6, SIGMOID, False, 3, 3, False, 1.0, 1, torch.float32),
+    (1100, 45, 4, SOFTMAX, True, 9, 4, True, 1.0, 16, torch.float32),
+    (400, 1000, 3, SIGMOID, True, 1, 1, True, 1.0, 1, torch.float16),
 ])
 def test_route(handle, t, e, k, score, with_bias, groups, top_groups, renorm, scale, align, dtype):
     gen = torch.Generator().manual_seed(t + e + k)
@@ -174,6 +176,17 @@ def test_route_masks(handle, score, groups, top_groups, with_bias):
     logits[10] = torch.where(torch.arange(32) % 8 == 0, logits[10], -math.inf)  # one expert in each group
     got = run_route(handle, logits, 4, score, bias, groups, top_groups, True, align=4)
     check_route(got, logits, 4, score, bias, groups, top_groups, True, 1.0, None, 4)
+
+
+@pytest.mark.parametrize("many", [2, 12, 50])
+def test_route_infinite_biases_come_first(handle, many):
+    """Experts with a bias of +inf tie at the top, in their order."""
+    gen = torch.Generator().manual_seed(many)
+    logits = torch.randn(100, 64, generator=gen)
+    bias = torch.randn(64, generator=gen) * 0.1
+    bias[torch.randperm(64, generator=gen)[:many]] = math.inf
+    got = run_route(handle, logits, 6, SIGMOID, bias, renorm=True)
+    check_route(got, logits, 6, SIGMOID, bias, 1, 1, True, 1.0, None, 1)
 
 
 @pytest.mark.parametrize("t,count", [(40, 0), (40, 7), (40, 400), (3000, 1234)])
