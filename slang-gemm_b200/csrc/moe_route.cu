@@ -19,6 +19,11 @@
 // timing): counts per block of tokens, then every block sums the counts of the
 // blocks before it and ranks its own slots. Few slots take one block and one
 // launch.
+//
+// Bound by instruction issue (about 1400 a token at 256 experts in 8 groups with a
+// bias and top_k 8, 600 without groups and bias): 16384 tokens take 48 us, 33 of
+// them the choice; 48 tokens of 64 experts take 9 us, the latency of one block. The
+// gradient of 16383 x 160 softmax logits takes 11 us.
 #include <type_traits>
 
 #include "gs_float.cuh"
