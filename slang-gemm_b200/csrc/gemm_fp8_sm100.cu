@@ -694,7 +694,12 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
 #pragma unroll
                         for (int b = 0; b < 128 / COLS; ++b) {
                             if (b * COLS >= n || p_warp >= it.p_end) break;
-                            if (lane == 0) bulk_wait_group_read<1>();  // of the store that last used this buffer
+                            // The store that last used this buffer has read it: the one before the last within a tile, any
+                            // of the tile before (a part tile's stores may be odd in number, and end on either buffer).
+                            if (lane == 0) {
+                                if (b == 0) bulk_wait_group_read<0>();
+                                else bulk_wait_group_read<1>();
+                            }
                             uint8_t *buf = stg + (ew * 2 + (b & 1)) * C_::STG_BLOCK;
                             const uint32_t dst = smem_u32(buf) + lane * 128;
                             __syncwarp();
