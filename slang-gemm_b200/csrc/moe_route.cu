@@ -232,7 +232,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
     const bool grouped = d.groups > 1 && d.top_groups < d.groups;
     Key key[VPL];
     bool close = false;
-    auto far = [&](float x, float y, float terms) { return !(fabsf(x - y) <= 2.0f * terms * doubt(d, x)); };
+    auto far = [&](float x, float y) { return !(fabsf(x - y) <= 2.0f * doubt(d, x)); };
     if (d.bias != nullptr || grouped) {
         R s[VPL];
         scores<R, VPL>(l, d.sigmoid != 0, top, s);
@@ -276,9 +276,14 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             }
             const bool kept = lane < d.groups && better < d.top_groups;
             if constexpr (F32) {
-                const Key worst = ~warp_max(kept ? ~mine : Key(0));
-                const Key best = warp_max(!kept && lane < d.groups ? mine : Key(0));
-                if (best > none && !far(value_of(worst), value_of(best), 2.0f)) close = true;
+                // How far the sum may be off: each of its two c by its own size, however small their sum, and the steps
+                // of the sum and of its limit. The least that a kept group may have has to pass the most that another may.
+                const bool live = k1 != none;
+                const float sum = value_of(mine);
+                const float reach = live ? doubt(d, value_of(k1)) + (k2 != none ? doubt(d, value_of(k2)) : 0.0f) + 2e-7f * fabsf(sum) : 0.0f;
+                const Key worst = ~warp_max(kept && live ? ~key_of(sum - reach) : Key(0));
+                const Key best = warp_max(!kept && live ? key_of(sum + reach) : Key(0));
+                if (best >= worst) close = true;
             }
             const uint32_t keep = __ballot_sync(kFull, kept);
 #pragma unroll
@@ -306,7 +311,7 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
         const Key m = warp_max(best);
         if (m == none) break;
         if constexpr (F32) {
-            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(m), 1.0f)) close = true;
+            if (d.bias != nullptr && j > 0 && !far(value_of(last), value_of(m))) close = true;
         }
         if (j == d.top_k) break;
         last = m;
