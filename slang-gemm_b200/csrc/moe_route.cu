@@ -278,11 +278,12 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             if constexpr (F32) {
                 // How far the sum may be off: each of its two c by its own size, however small their sum, and the steps
                 // of the sum and of its limit. The least that a kept group may have has to pass the most that another may.
+                // A sum beyond f32's range may be anything (its limits are NaN, or infinite).
                 const bool live = k1 != none;
                 const float sum = value_of(mine);
                 const float reach = live ? doubt(d, value_of(k1)) + (k2 != none ? doubt(d, value_of(k2)) : 0.0f) + 2e-7f * fabsf(sum) : 0.0f;
-                const Key worst = ~warp_max(kept && live ? ~key_of(sum - reach) : Key(0));
-                const Key best = warp_max(!kept && live ? key_of(sum + reach) : Key(0));
+                const Key worst = ~warp_max(kept && live ? ~key_of(fmaxf(sum - reach, -INFINITY)) : Key(0));
+                const Key best = warp_max(!kept && live ? key_of(fminf(sum + reach, INFINITY)) : Key(0));
                 if (best >= worst) close = true;
             }
             const uint32_t keep = __ballot_sync(kFull, kept);
