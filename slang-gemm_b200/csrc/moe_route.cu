@@ -24,6 +24,7 @@
 // bias and top_k 8, 600 without groups and bias): 16384 tokens take 48 us, 33 of
 // them the choice; 48 tokens of 64 experts take 9 us, the latency of one block. The
 // gradient of 16383 x 160 softmax logits takes 11 us.
+#include <atomic>
 #include <type_traits>
 
 #include "gs_float.cuh"
@@ -606,18 +607,33 @@ __global__ void __launch_bounds__(kPlanThreads) k_route_plan(const __grid_consta
     fill_padding<kPlanThreads>(d, count, base, blockIdx.x, blocks);
 }
 
+// Dynamic shared memory of the kernels that make a plan: count, bases and every warp's counters; the plan kernel's own
+// counts besides.
+constexpr size_t plan_bytes(bool small, int experts) {
+    return (static_cast<size_t>(experts | 1) * (small ? kWarps : kPlanThreads / 32) + static_cast<size_t>(experts) * (small ? 2 : 3) + 1) * sizeof(int);
+}
+
+// Opts `kern` in to the most shared memory that any of its calls needs, once per device: the limit is the kernel's for
+// all threads, so one that followed each call's size would change between another thread's setting and its launch.
+// `done` is the kernel's own.
+template <typename K>
+static cudaError_t allow_shared(Context &ctx, K kern, size_t most, std::atomic<bool> (&done)[64]) {
+    const bool known = ctx.device >= 0 && ctx.device < 64;
+    if (most <= 32 * 1024 || (known && done[ctx.device].load(std::memory_order_relaxed))) return cudaSuccess;  // with the static arrays within the 48 KiB that need no opt-in
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+    if (e == cudaSuccess && known) done[ctx.device].store(true, std::memory_order_relaxed);
+    return e;
+}
+
 template <typename T, int VPL>
 static cudaError_t launch(Context &ctx, const RouteDesc &d) {
+    static std::atomic<bool> small_set[64], plan_set[64];
     const int blocks = route_blocks(d.tokens, d.top_k);
-    // count, bases and every warp's counters; the plan kernel's own counts besides
-    const size_t smem = (static_cast<size_t>(d.experts | 1) * (blocks == 0 ? kWarps : kPlanThreads / 32) + static_cast<size_t>(d.experts) * (blocks == 0 ? 2 : 3) + 1) * sizeof(int);
-    if (smem > 32 * 1024) {  // with the static arrays past the 48 KiB that need no opt-in
-        const cudaError_t e = blocks == 0 ? cudaFuncSetAttribute(k_route_small<T, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))
-                                          : cudaFuncSetAttribute(k_route_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-    }
+    const size_t smem = d.offsets != nullptr ? plan_bytes(blocks == 0, d.experts) : 0;
     if (blocks == 0) {
-        const cudaError_t e = launch_pdl(k_route_small<T, VPL>, dim3(1), dim3(kThreads), smem, ctx.stream, 1, d);
+        cudaError_t e = allow_shared(ctx, k_route_small<T, VPL>, plan_bytes(true, VPL * 32), small_set);
+        if (e != cudaSuccess) return e;
+        e = launch_pdl(k_route_small<T, VPL>, dim3(1), dim3(kThreads), smem, ctx.stream, 1, d);
         ctx.launches++;
         return e;
     }
@@ -626,6 +642,8 @@ static cudaError_t launch(Context &ctx, const RouteDesc &d) {
                                static_cast<size_t>(d.experts) * sizeof(int), ctx.stream, 1, d, per);
     ctx.launches++;
     if (e != cudaSuccess || d.offsets == nullptr) return e;
+    e = allow_shared(ctx, k_route_plan, plan_bytes(false, GS_ROUTE_MAX_EXPERTS), plan_set);
+    if (e != cudaSuccess) return e;
     e = launch_pdl(k_route_plan, dim3(static_cast<unsigned>(blocks)), dim3(kPlanThreads), smem, ctx.stream, 1, d, per);
     ctx.launches++;
     return e;
