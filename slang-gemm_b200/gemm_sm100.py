@@ -359,8 +359,13 @@ class Handle:
 
     # ---- handle state ----
     def set_stream(self, stream):
-        """stream: a torch.cuda.Stream, a raw cudaStream_t int, or None."""
-        self._check(_fast.set_stream(self._raw, getattr(stream, "cuda_stream", stream)), "gs_set_stream")
+        """stream: a torch.cuda.Stream, a raw cudaStream_t (an int or a ctypes.c_void_p), or None."""
+        ptr = getattr(stream, "cuda_stream", stream)
+        if isinstance(ptr, ctypes.c_void_p):
+            ptr = ptr.value
+        elif ptr is not None and not isinstance(ptr, int):  # the binding would take a tensor's address
+            raise TypeError(f"not a CUDA stream: {type(stream).__name__}")
+        self._check(_fast.set_stream(self._raw, ptr), "gs_set_stream")
 
     def last_error(self) -> str:
         return _lib.gs_last_error(self._h).decode()
