@@ -9,12 +9,14 @@ CUDA tensors. `host_gemm_ex` mirrors `gemm.gemmEx` (src/gemm.zig:546) over
 host numpy buffers.
 
 There is no CPU fallback: importing this module fails if the shared library
-(and `_gs_fastcall`, the native binding of the FP8 and routed-expert calls) has
-not been built, and every call fails without an sm_100 device.
+has not been built, and every call fails without an sm_100 device. The FP8 and
+routed-expert calls go through a native module, `_gs_fastcall`, where the build
+had this Python's headers, and through ctypes (about 3 us a call more) elsewhere.
 """
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 from dataclasses import dataclass
 
@@ -199,7 +201,78 @@ def _load() -> ctypes.CDLL:
 
 _lib = _load()
 
-import _gs_fastcall as _fast  # noqa: E402  (needs the library; built beside it by the same make)
+
+def _ptr(x) -> int | None:
+    """Device pointer of a torch tensor, or an int / None passed through."""
+    if x is None:
+        return None
+    if isinstance(x, int):
+        return x
+    return x.data_ptr()
+
+
+class _CtypesCalls:
+    """What `_gs_fastcall` has, with its arguments and its refusals, through ctypes."""
+
+    @staticmethod
+    def _convert(name, kinds, args):
+        if len(args) != len(kinds):
+            raise TypeError(f"{name} takes {len(kinds)} arguments, got {len(args)}")
+        out = []
+        for at, (kind, a) in enumerate(zip(kinds, args)):
+            if kind is ctypes.c_void_p:
+                out.append(_ptr(a))
+            elif kind is ctypes.c_float:
+                out.append(float(a))
+            else:
+                v = operator.index(a)
+                if kind is ctypes.c_int and not -2 ** 31 <= v < 2 ** 31:
+                    raise OverflowError(f"argument {at} of {name} does not fit a C int")
+                out.append(v)
+        return out
+
+    @classmethod
+    def _call(cls, name, scalars=()):
+        """scalars: positions of alpha and beta, which the library takes by address."""
+        fn = getattr(_lib, "gs_" + name)
+        kinds = [ctypes.c_float if at in scalars else kind for at, kind in enumerate(fn.argtypes)]
+
+        def call(*args):
+            v = cls._convert(name, kinds, args)
+            for at in scalars:
+                v[at] = ctypes.byref(ctypes.c_float(v[at]))
+            return fn(*v)
+
+        return call
+
+    @classmethod
+    def _route_call(cls, name):
+        """gs_route_desc's fields stand in the place of the descriptor."""
+        fn = getattr(_lib, "gs_" + name)
+        fields = [kind for _, kind in RouteDesc._fields_]
+        kinds = [ctypes.c_void_p, *fields, *fn.argtypes[2:]]
+        end = 1 + len(fields)
+
+        def call(*args):
+            v = cls._convert(name, kinds, args)
+            return fn(v[0], ctypes.byref(RouteDesc(*v[1:end])), *v[end:])
+
+        return call
+
+    def __init__(self):
+        self.__name__ = "ctypes"
+        for name in ("set_stream", "fp8_quantize", "moe_combine", "moe_combine_backward"):
+            setattr(self, name, self._call(name))
+        self.gemm_fp8 = self._call("gemm_fp8", (6, 19))
+        self.gemm_fp8_grouped = self._call("gemm_fp8_grouped", (9, 24))
+        self.moe_route = self._route_call("moe_route")
+        self.moe_route_backward = self._route_call("moe_route_backward")
+
+
+try:
+    import _gs_fastcall as _fast  # noqa: E402  (needs the library; built beside it by the same make)
+except ImportError:  # no Python headers at the build, or another Python's
+    _fast = _CtypesCalls()
 
 
 def lib() -> ctypes.CDLL:
@@ -280,15 +353,6 @@ def moe_route_workspace(tokens: int, experts: int, top_k: int) -> int:
     if s != STATUS_SUCCESS:
         raise GemmError(s, "gs_moe_route_workspace")
     return out.value
-
-
-def _ptr(x) -> int | None:
-    """Device pointer of a torch tensor, or an int / None passed through."""
-    if x is None:
-        return None
-    if isinstance(x, int):
-        return x
-    return x.data_ptr()
 
 
 def _scalar(compute: int, v):
