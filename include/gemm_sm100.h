@@ -92,6 +92,8 @@ gs_status gs_destroy(gs_handle handle);
 /* stream is a cudaStream_t (NULL = legacy default stream). */
 gs_status gs_set_stream(gs_handle handle, void *stream);
 gs_status gs_get_stream(gs_handle handle, void **stream);
+/* Index of the CUDA device the handle was created on. */
+gs_status gs_get_device(gs_handle handle, int *device);
 /* Static, NUL-terminated name of a status value. */
 const char *gs_status_name(gs_status status);
 /* Human-readable detail of the last non-success status returned on this handle. */

@@ -220,6 +220,12 @@ gs_status gs_get_stream(gs_handle h, void **stream) {
     *stream = h->ctx.stream;
     return GS_STATUS_SUCCESS;
 }
+gs_status gs_get_device(gs_handle h, int *device) {
+    if (!h) return GS_STATUS_NOT_INITIALIZED;
+    if (!device) return GS_STATUS_INVALID_VALUE;
+    *device = h->ctx.device;
+    return GS_STATUS_SUCCESS;
+}
 
 const char *gs_last_error(gs_handle h) { return h ? h->ctx.last_error.c_str() : "null handle"; }
 uint32_t gs_last_kernels(gs_handle h) { return h ? h->ctx.last_kernels : 0u; }

@@ -147,6 +147,7 @@ def _load() -> ctypes.CDLL:
         "gs_destroy": (st, [vp]),
         "gs_set_stream": (st, [vp, vp]),
         "gs_get_stream": (st, [vp, ctypes.POINTER(vp)]),
+        "gs_get_device": (st, [vp, ctypes.POINTER(i)]),
         "gs_status_name": (ctypes.c_char_p, [i]),
         "gs_last_error": (ctypes.c_char_p, [vp]),
         "gs_last_kernels": (u32, [vp]),
@@ -430,6 +431,13 @@ class Handle:
         elif ptr is not None and not isinstance(ptr, int):  # the binding would take a tensor's address
             raise TypeError(f"not a CUDA stream: {type(stream).__name__}")
         self._check(_fast.set_stream(self._raw, ptr), "gs_set_stream")
+
+    @property
+    def device(self) -> str:
+        """The device the handle is bound to, as torch names it ("cuda:0")."""
+        d = ctypes.c_int(-1)
+        self._check(_lib.gs_get_device(self._h, ctypes.byref(d)), "gs_get_device")
+        return f"cuda:{d.value}"
 
     def last_error(self) -> str:
         return _lib.gs_last_error(self._h).decode()

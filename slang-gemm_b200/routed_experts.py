@@ -28,7 +28,7 @@ def _blocks(n: int) -> int:
 class RoutedExperts:
     """tokens, experts, top_k: the routing's sizes; d_in, d_out: the experts' (multiples of 16). align 128 is what the
     weight gradient needs; 1 wastes no rows and is for serving (no backward). score, bias, groups, top_groups and scale
-    are moe_route's."""
+    are moe_route's. The buffers are on the handle's device."""
 
     def __init__(self, handle, tokens, experts, top_k, d_in, d_out, align=128, score=gs.ROUTE_SOFTMAX, bias=None,
                  groups=1, top_groups=1, renormalize=True, scale=1.0, token_count=None, weights_of=None):
@@ -39,8 +39,9 @@ class RoutedExperts:
         self.routing = dict(bias=bias, score=score, groups=groups, top_groups=top_groups, renormalize=renormalize,
                             scale=scale, token_count=token_count)
         self.rows = rows = gs.moe_rows(tokens, experts, top_k, align)
-        i32, u8, f32 = (dict(dtype=t, device="cuda") for t in (torch.int32, torch.uint8, torch.float32))
-        bf16 = dict(dtype=torch.bfloat16, device="cuda")
+        self.device = torch.device(handle.device)
+        i32, u8, f32, bf16 = (dict(dtype=t, device=self.device)
+                              for t in (torch.int32, torch.uint8, torch.float32, torch.bfloat16))
         self.ids, self.p = torch.empty(tokens, top_k, **i32), torch.empty(tokens, top_k, **f32)
         self.slot_row, self.row_slot = torch.empty(tokens, top_k, **i32), torch.empty(rows, **i32)
         self.offsets = torch.empty(experts + 1, **i32)
@@ -60,7 +61,7 @@ class RoutedExperts:
         if self._grad is None:
             if self.align % 128:
                 raise ValueError("backward needs a plan aligned to 128 rows")
-            f32, u8 = dict(device="cuda"), dict(dtype=torch.uint8, device="cuda")
+            f32, u8, bf16 = (dict(dtype=t, device=self.device) for t in (torch.float32, torch.uint8, torch.bfloat16))
             r, rb = self.rows, _blocks(self.rows)
             self._grad = dict(
                 dy=torch.empty_like(self.y), dp=torch.empty_like(self.p),
@@ -68,8 +69,7 @@ class RoutedExperts:
                 gq=torch.empty(r, self.d_out, **u8), g_scale=torch.empty(_blocks(self.d_out), r, **f32),
                 gtq=torch.empty(r, self.d_out, **u8), gt_scale=torch.empty(rb, self.d_out, **f32),
                 xtq=torch.empty(r, self.d_in, **u8), xt_scale=torch.empty(rb, self.d_in, **f32),
-                dx_rows=torch.zeros(r, self.d_in, dtype=torch.bfloat16, device="cuda"),
-                dx=torch.empty(self.tokens, self.d_in, dtype=torch.bfloat16, device="cuda"),
+                dx_rows=torch.zeros(r, self.d_in, **bf16), dx=torch.empty(self.tokens, self.d_in, **bf16),
                 dw=torch.empty(self.experts, self.d_out, self.d_in, **f32))
         return self._grad
 
