@@ -25,6 +25,18 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
+def _rows(name, t, dtype, rows, cols, device):
+    """The leading dimension of t, a rows x cols matrix as the kernels read it; ValueError if it is another. Looks at no
+    value, so it may run under capture."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows, cols) or t.device != device:
+        got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] on {device}, not {got}")
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or (ld < cols and rows > 1):
+        raise ValueError(f"{name}'s rows must be contiguous and must not overlap; its strides are {t.stride()}")
+    return ld if rows > 1 else cols
+
+
 class RoutedExperts:
     """tokens, experts, top_k: the routing's sizes; d_in, d_out: the experts' (multiples of 16). align 128 is what the
     weight gradient needs; 1 wastes no rows and is for serving (no backward). score, bias, groups, top_groups and scale
@@ -81,12 +93,16 @@ class RoutedExperts:
                                 gs.R_8F_E4M3, self.d_in, self.w_scale[e], _blocks(self.d_in))
 
     def forward(self, x, logits):
-        """x: [tokens, d_in] bf16, logits: [tokens, experts] f32. Returns out [tokens, d_out] bf16 (the layer's buffer)."""
+        """x: [tokens, d_in] bf16, logits: [tokens, experts] f32, each with contiguous rows (which may lie apart); a batch of
+        fewer tokens is padded to `tokens` rows and counted by token_count. Returns out [tokens, d_out] bf16 (the layer's
+        buffer)."""
         h, i, o, rows = self.h, self.d_in, self.d_out, self.rows
-        h.moe_route(self.tokens, self.experts, self.top_k, logits, gs.R_32F, self.experts, self.ids, self.p,
+        ldx = _rows("x", x, torch.bfloat16, self.tokens, i, self.device)
+        ldl = _rows("logits", logits, torch.float32, self.tokens, self.experts, self.device)
+        h.moe_route(self.tokens, self.experts, self.top_k, logits, gs.R_32F, ldl, self.ids, self.p,
                     align=self.align, offsets=self.offsets, slot_row=self.slot_row, row_slot=self.row_slot, rows=rows,
                     workspace=self._ws, workspace_bytes=self._ws_bytes, **self.routing)
-        h.fp8_quantize(gs.SCALE_VEC128, 0, i, rows, x, gs.R_16BF, i, self.xq, gs.R_8F_E4M3, i, self.x_scale, rows,
+        h.fp8_quantize(gs.SCALE_VEC128, 0, i, rows, x, gs.R_16BF, ldx, self.xq, gs.R_8F_E4M3, i, self.x_scale, rows,
                        index=self.row_slot, index_div=self.top_k, src_cols=self.tokens)
         h.gemm_fp8_grouped(gs.GROUP_N, gs.OP_T, gs.OP_N, o, rows, i, self.experts, self.offsets, 1.0, self.wq,
                            gs.R_8F_E4M3, i, o * i, self.w_scale, gs.SCALE_BLK128, _blocks(i), _blocks(i) * _blocks(o),
@@ -96,17 +112,21 @@ class RoutedExperts:
         return self.out
 
     def backward(self, x, logits, dout):
-        """Gradients of the last forward for dout [tokens, d_out] bf16: dx [tokens, d_in] bf16, dlogits f32, dw
-        [experts, d_out, d_in] f32 (buffers of the layer)."""
-        h, i, o, rows, b = self.h, self.d_in, self.d_out, self.rows, self._gradient_buffers()
+        """Gradients of the last forward, for its x and logits and dout [tokens, d_out] bf16: dx [tokens, d_in] bf16, dlogits
+        f32, dw [experts, d_out, d_in] f32 (buffers of the layer)."""
+        h, i, o, rows = self.h, self.d_in, self.d_out, self.rows
+        ldx = _rows("x", x, torch.bfloat16, self.tokens, i, self.device)
+        ldl = _rows("logits", logits, torch.float32, self.tokens, self.experts, self.device)
+        ldg = _rows("dout", dout, torch.bfloat16, self.tokens, o, self.device)
+        b = self._gradient_buffers()
         h.moe_combine_backward(self.tokens, self.top_k, o, self.y, gs.R_16BF, o, rows, self.slot_row, self.row_slot,
-                               self.p, dout, gs.R_16BF, o, b["dy"], o, b["dp"])
-        h.moe_route_backward(self.tokens, self.experts, self.top_k, logits, gs.R_32F, self.experts, self.ids, b["dp"],
+                               self.p, dout, gs.R_16BF, ldg, b["dy"], o, b["dp"])
+        h.moe_route_backward(self.tokens, self.experts, self.top_k, logits, gs.R_32F, ldl, self.ids, b["dp"],
                              b["dlogits"], gs.R_32F, self.experts, score=self.routing["score"],
                              renormalize=self.routing["renormalize"], scale=self.routing["scale"])
         h.fp8_quantize(gs.SCALE_VEC128, 0, o, rows, b["dy"], gs.R_16BF, o, b["gq"], gs.R_8F_E5M2, o, b["g_scale"], rows)
         h.fp8_quantize(gs.SCALE_VEC128, 1, o, rows, b["dy"], gs.R_16BF, o, b["gtq"], gs.R_8F_E5M2, o, b["gt_scale"], o)
-        h.fp8_quantize(gs.SCALE_VEC128, 1, i, rows, x, gs.R_16BF, i, b["xtq"], gs.R_8F_E4M3, i, b["xt_scale"], i,
+        h.fp8_quantize(gs.SCALE_VEC128, 1, i, rows, x, gs.R_16BF, ldx, b["xtq"], gs.R_8F_E4M3, i, b["xt_scale"], i,
                        index=self.row_slot, index_div=self.top_k, src_cols=self.tokens)
         h.gemm_fp8_grouped(gs.GROUP_N, gs.OP_N, gs.OP_N, i, rows, o, self.experts, self.offsets, 1.0, self.wq,
                            gs.R_8F_E4M3, i, o * i, self.w_scale, gs.SCALE_BLK128, _blocks(i), _blocks(i) * _blocks(o),

@@ -43,3 +43,86 @@ def test_a_handle_names_its_device(cuda):
         assert h.device == "cuda:0"
         l = layer(h)
         assert {t.device for t in tensors(l)} == {torch.device("cuda", 0)}
+
+
+def inputs(tokens=5, experts=4, d_in=32, d_out=48):
+    return (torch.zeros(tokens, d_in, dtype=torch.bfloat16), torch.zeros(tokens, experts),
+            torch.zeros(tokens, d_out, dtype=torch.bfloat16))
+
+
+X = {
+    "f32": lambda x: x.float(), "f16": lambda x: x.half(), "short": lambda x: x[:4], "long": lambda x: torch.cat([x, x]),
+    "narrow": lambda x: x[:, :-1], "flat": lambda x: x.reshape(-1), "transposed": lambda x: x.t().contiguous().t(),
+    "expanded": lambda x: x[:1].expand_as(x), "every second column": lambda x: torch.cat([x, x], 1)[:, ::2],
+    "overlapping rows": lambda x: torch.as_strided(x, x.shape, (1, 1)), "another device": lambda x: x.to("meta"),
+    "none": lambda x: None, "nested list": lambda x: x.tolist(),
+}
+
+
+@pytest.mark.parametrize("change", [k for k in X])
+@pytest.mark.parametrize("which", ["x", "logits", "dout"])
+def test_inputs_that_the_kernels_would_read_wrongly_are_refused(which, change):
+    h = FakeHandle()
+    l = layer(h)
+    good = dict(zip(("x", "logits", "dout"), inputs()))
+    l.forward(good["x"], good["logits"])
+    l.backward(**good)
+    if which == "logits" and change == "f32":
+        change = "f16"
+    bad = dict(good, **{which: X[change](good[which])})
+    h.calls.clear()
+    if which != "dout":
+        with pytest.raises(ValueError, match=which):
+            l.forward(bad["x"], bad["logits"])
+    with pytest.raises(ValueError, match=which):
+        l.backward(**bad)
+    assert not h.calls  # refused before anything is launched
+
+
+def test_rows_may_lie_apart():
+    """A slice of a wider tensor: its leading dimension reaches the library."""
+    h = FakeHandle()
+    l = layer(h)
+    wide = [torch.zeros(5, n, dtype=t)[:, 8:] for n, t in ((32 + 8, torch.bfloat16), (4 + 8, torch.float32), (48 + 8, torch.bfloat16))]
+    l.forward(*wide[:2])
+    l.backward(*wide)
+    calls = {}
+    for name, args, _ in h.calls:
+        calls.setdefault(name, []).append(args)
+    for args in calls["moe_route"] + calls["moe_route_backward"]:
+        assert args[3] is wide[1] and args[5] == 12
+    casts = [args for args in calls["fp8_quantize"] if args[4] is wide[0]]
+    assert len(casts) == 2 and all(args[6] == 40 for args in casts)
+    (args,) = calls["moe_combine_backward"]
+    assert args[10] is wide[2] and args[12] == 56
+
+
+def test_one_token_may_have_any_row_stride():
+    l = layer(tokens=1)
+    x, logits, dout = (torch.as_strided(t, t.shape, (1, 1)) for t in inputs(1))
+    l.forward(x, logits)
+    l.backward(x, logits, dout)
+    assert [args[5] for name, args, _ in l.h.calls if name == "moe_route"] == [4]
+
+
+@pytest.mark.gpu
+def test_slices_of_wider_tensors_give_the_same_results(cuda):
+    gen = torch.Generator().manual_seed(4)
+    x, logits, dout = (torch.randn(150, n, generator=gen).to(t).cuda()
+                       for n, t in ((256, torch.bfloat16), (6, torch.float32), (384, torch.bfloat16)))
+    with gs.Handle() as h:
+        l = layer(h, 150, 6, 2, 256, 384)
+        l.set_weights(torch.randn(6, 384, 256, generator=gen).cuda())
+
+        def outputs(*args):
+            out = l.forward(*args[:2]).clone()
+            grads = [g.clone() for g in l.backward(*args)]
+            torch.cuda.synchronize()
+            assert h.device_error() == 0
+            return [out, *grads]
+
+        whole = outputs(x, logits, dout)
+        for left, right in ((8, 8), (3, 2)):  # 16-byte aligned rows, and odd ones
+            wide = [torch.cat([t.new_full((150, left), 7), t, t.new_full((150, right), 7)], 1)[:, left:-right] for t in (x, logits, dout)]
+            for a, b in zip(whole, outputs(*wide)):
+                assert torch.equal(a, b)
