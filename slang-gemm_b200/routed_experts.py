@@ -29,12 +29,22 @@ def _rows(name, t, dtype, rows, cols, device):
     """The leading dimension of t, a rows x cols matrix as the kernels read it; ValueError if it is another. Looks at no
     value, so it may run under capture."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows, cols) or t.device != device:
-        got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] on {device}, not {got}")
+        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] on {device}, not {_describe(t)}")
     ld, step = t.stride()
     if (step != 1 and cols > 1) or (ld < cols and rows > 1):
         raise ValueError(f"{name}'s rows must be contiguous and must not overlap; its strides are {t.stride()}")
     return ld if rows > 1 else cols
+
+
+def _describe(t) -> str:
+    return f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+
+
+def _vector(name, t, dtype, shapes, device):
+    """ValueError unless t is None or contiguous, of one of `shapes`."""
+    if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) in shapes and
+                              t.device == device and t.is_contiguous()):
+        raise ValueError(f"{name} must be {dtype} {list(shapes[0])} on {device}, contiguous, not {_describe(t)}")
 
 
 class RoutedExperts:
@@ -44,6 +54,8 @@ class RoutedExperts:
 
     def __init__(self, handle, tokens, experts, top_k, d_in, d_out, align=128, score=gs.ROUTE_SOFTMAX, bias=None,
                  groups=1, top_groups=1, renormalize=True, scale=1.0, token_count=None, weights_of=None):
+        if tokens < 1 or d_in < 1 or d_out < 1:
+            raise ValueError("tokens, d_in and d_out must be positive")
         if d_in % 16 or d_out % 16:
             raise ValueError("d_in and d_out must be multiples of 16 (16-byte aligned FP8 rows)")
         self.h, self.tokens, self.experts, self.top_k = handle, tokens, experts, top_k
@@ -52,6 +64,8 @@ class RoutedExperts:
                             scale=scale, token_count=token_count)
         self.rows = rows = gs.moe_rows(tokens, experts, top_k, align)
         self.device = torch.device(handle.device)
+        _vector("bias", bias, torch.float32, [(experts,)], self.device)
+        _vector("token_count", token_count, torch.int32, [(1,), ()], self.device)
         i32, u8, f32, bf16 = (dict(dtype=t, device=self.device)
                               for t in (torch.int32, torch.uint8, torch.float32, torch.bfloat16))
         self.ids, self.p = torch.empty(tokens, top_k, **i32), torch.empty(tokens, top_k, **f32)
@@ -60,6 +74,9 @@ class RoutedExperts:
         self._ws_bytes = gs.moe_route_workspace(tokens, experts, top_k)
         self._ws = torch.empty(max(self._ws_bytes, 4), **u8)
         ki, ko = _blocks(d_in), _blocks(d_out)
+        if weights_of is not None and ((weights_of.experts, weights_of.d_in, weights_of.d_out, weights_of.device) !=
+                                       (experts, d_in, d_out, self.device)):
+            raise ValueError("weights_of must be a layer with the same experts, d_in and d_out on the same device")
         if weights_of is None:
             self.wq, self.w_scale = torch.empty(experts, d_out, d_in, **u8), torch.empty(experts, ko, ki, **f32)
         else:
@@ -86,8 +103,15 @@ class RoutedExperts:
         return self._grad
 
     def set_weights(self, w):
-        """w: [experts, d_out, d_in] f32, f16 or bf16; cast to FP8 blocks."""
-        wt = {torch.float32: gs.R_32F, torch.float16: gs.R_16F, torch.bfloat16: gs.R_16BF}[w.dtype]
+        """w: [experts, d_out, d_in] f32, f16 or bf16 with contiguous rows (which may lie apart); cast to FP8 blocks."""
+        types = {torch.float32: gs.R_32F, torch.float16: gs.R_16F, torch.bfloat16: gs.R_16BF}
+        if (not isinstance(w, torch.Tensor) or w.dtype not in types or w.shape != (self.experts, self.d_out, self.d_in) or
+                w.device != self.device):
+            raise ValueError(f"w must be f32, f16 or bf16 [{self.experts}, {self.d_out}, {self.d_in}] on {self.device}, "
+                             f"not {_describe(w)}")
+        if w.stride(2) != 1 or w.stride(1) < self.d_in:
+            raise ValueError(f"w's rows must be contiguous and must not overlap; its strides are {w.stride()}")
+        wt = types[w.dtype]
         for e in range(self.experts):
             self.h.fp8_quantize(gs.SCALE_BLK128, 0, self.d_in, self.d_out, w[e], wt, w.stride(1), self.wq[e],
                                 gs.R_8F_E4M3, self.d_in, self.w_scale[e], _blocks(self.d_in))

@@ -126,3 +126,71 @@ def test_slices_of_wider_tensors_give_the_same_results(cuda):
             wide = [torch.cat([t.new_full((150, left), 7), t, t.new_full((150, right), 7)], 1)[:, left:-right] for t in (x, logits, dout)]
             for a, b in zip(whole, outputs(*wide)):
                 assert torch.equal(a, b)
+
+
+W = {
+    "f64": lambda w: w.double(), "fp8": lambda w: w.to(torch.float8_e4m3fn), "transposed": lambda w: w.transpose(1, 2).contiguous().transpose(1, 2),
+    "[in, out]": lambda w: w.transpose(1, 2), "short": lambda w: w[:3], "long": lambda w: torch.cat([w, w]),
+    "wide": lambda w: torch.cat([w, w], 2), "expanded rows": lambda w: w[:, :1].expand_as(w), "flat": lambda w: w.reshape(-1),
+    "another device": lambda w: w.to("meta"), "list": lambda w: list(w),
+}
+
+
+@pytest.mark.parametrize("change", [k for k in W])
+def test_weights_that_would_be_read_wrongly_are_refused(change):
+    l = layer()
+    with pytest.raises(ValueError, match="w"):
+        l.set_weights(W[change](torch.zeros(4, 48, 32)))
+    assert not l.h.calls
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, gs.R_32F), (torch.float16, gs.R_16F), (torch.bfloat16, gs.R_16BF)])
+def test_weights_may_lie_apart(dtype, code):
+    l = layer()
+    w = torch.zeros(8, 50, 40, dtype=dtype)[::2, 1:49, 8:]
+    l.set_weights(w)
+    assert [(args[4].data_ptr(), args[5], args[6]) for _, args, _ in l.h.calls] == [(w[e].data_ptr(), code, 40) for e in range(4)]
+
+
+@pytest.mark.parametrize("sizes", [dict(experts=5), dict(d_in=48), dict(d_out=32)])
+def test_weights_of_another_size_are_refused(sizes):
+    other = layer(**sizes)
+    with pytest.raises(ValueError, match="weights_of"):
+        layer(weights_of=other)
+
+
+def test_weights_of_another_device_are_refused():
+    class Elsewhere(FakeHandle):
+        device = "meta"
+
+    with pytest.raises(ValueError, match="weights_of"):
+        layer(weights_of=layer(Elsewhere()))
+
+
+def test_weights_can_be_shared_by_layers_of_other_batches():
+    first = layer()
+    second = layer(tokens=9, top_k=1, align=1, weights_of=first)
+    assert second.wq is first.wq and second.w_scale is first.w_scale
+
+
+@pytest.mark.parametrize("name,value", [
+    ("bias", torch.zeros(5)), ("bias", torch.zeros(4, dtype=torch.bfloat16)), ("bias", torch.zeros(8)[::2]),
+    ("bias", torch.zeros(4, 1)), ("bias", torch.zeros(4, device="meta")), ("bias", [0.0] * 4),
+    ("token_count", torch.tensor([3])), ("token_count", torch.tensor([3.0])), ("token_count", torch.tensor([], dtype=torch.int32)),
+    ("token_count", torch.tensor([3, 4], dtype=torch.int32)), ("token_count", torch.tensor([3], dtype=torch.int32, device="meta")),
+    ("token_count", 3),
+])
+def test_routing_tensors_that_would_be_read_wrongly_are_refused(name, value):
+    with pytest.raises(ValueError, match=name):
+        layer(**{name: value})
+
+
+def test_routing_tensors_that_fit():
+    layer(bias=torch.zeros(4), token_count=torch.tensor([3], dtype=torch.int32))
+    layer(token_count=torch.tensor(3, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("sizes", [dict(tokens=0), dict(tokens=-1), dict(d_in=0), dict(d_out=-16), dict(d_in=24), dict(d_out=40)])
+def test_sizes_that_no_call_takes_are_refused(sizes):
+    with pytest.raises(ValueError):
+        layer(**sizes)
