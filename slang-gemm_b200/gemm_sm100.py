@@ -439,6 +439,13 @@ class Handle:
         self._check(_lib.gs_get_device(self._h, ctypes.byref(d)), "gs_get_device")
         return f"cuda:{d.value}"
 
+    @property
+    def stream(self) -> int:
+        """The handle's stream, a raw cudaStream_t (0: the legacy default stream)."""
+        p = ctypes.c_void_p()
+        self._check(_lib.gs_get_stream(self._h, ctypes.byref(p)), "gs_get_stream")
+        return p.value or 0
+
     def last_error(self) -> str:
         return _lib.gs_last_error(self._h).decode()
 

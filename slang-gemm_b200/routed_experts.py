@@ -10,9 +10,16 @@ gradient is the grouped product with the same weight blocks read the other way,
 the weight gradient the grouped product over each expert's tokens, both operands
 cast in vectors along the tokens.
 
-Nothing synchronises or allocates after construction, so both can be captured
-into a CUDA graph. An instance serves one stream at a time; concurrent use needs
-an instance each (the weight blocks can be shared by passing `weights_of`).
+The buffers are made by the constructor and, the gradients' larger ones, by
+`prepare_backward` (or else the first backward): torch allocates them, and where
+torch's current stream is not the handle's, the call waits for that stream, which
+may still use the memory. After that nothing synchronises or allocates, so both
+directions can be captured into a CUDA graph.
+
+All kernels run on the handle's stream: the caller orders the inputs' making before
+them and the outputs' use, or the layer's end, after them. An instance serves one
+stream at a time; concurrent use needs an instance each (the weight blocks can be
+shared by passing `weights_of`).
 """
 from __future__ import annotations
 
@@ -82,14 +89,24 @@ class RoutedExperts:
         else:
             self.wq, self.w_scale = weights_of.wq, weights_of.w_scale
         self.xq, self.x_scale = torch.empty(rows, d_in, **u8), torch.empty(ki, rows, **f32)
-        self.y = torch.zeros(rows, d_out, **bf16)  # rows behind the last expert's are never written
+        self.y = torch.empty(rows, d_out, **bf16)  # rows behind the last expert's are neither written nor read
         self.out = torch.empty(tokens, d_out, **bf16)
         self._grad = None
+        self._settle()
 
-    def _gradient_buffers(self):
+    def _settle(self):
+        """New memory may still be in use on the stream it was allocated on; the kernels that write it are on the handle's."""
+        if self.device.type != "cuda" or torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.device)
+        if current.cuda_stream != self.h.stream:
+            current.synchronize()
+
+    def prepare_backward(self):
+        """Makes the gradients' buffers, if they are not there: to be called before a capture, or a time that counts."""
+        if self.align % 128:
+            raise ValueError("backward needs a plan aligned to 128 rows")
         if self._grad is None:
-            if self.align % 128:
-                raise ValueError("backward needs a plan aligned to 128 rows")
             f32, u8, bf16 = (dict(dtype=t, device=self.device) for t in (torch.float32, torch.uint8, torch.bfloat16))
             r, rb = self.rows, _blocks(self.rows)
             self._grad = dict(
@@ -98,9 +115,9 @@ class RoutedExperts:
                 gq=torch.empty(r, self.d_out, **u8), g_scale=torch.empty(_blocks(self.d_out), r, **f32),
                 gtq=torch.empty(r, self.d_out, **u8), gt_scale=torch.empty(rb, self.d_out, **f32),
                 xtq=torch.empty(r, self.d_in, **u8), xt_scale=torch.empty(rb, self.d_in, **f32),
-                dx_rows=torch.zeros(r, self.d_in, **bf16), dx=torch.empty(self.tokens, self.d_in, **bf16),
+                dx_rows=torch.empty(r, self.d_in, **bf16), dx=torch.empty(self.tokens, self.d_in, **bf16),
                 dw=torch.empty(self.experts, self.d_out, self.d_in, **f32))
-        return self._grad
+            self._settle()
 
     def set_weights(self, w):
         """w: [experts, d_out, d_in] f32, f16 or bf16 with contiguous rows (which may lie apart); cast to FP8 blocks."""
@@ -142,7 +159,8 @@ class RoutedExperts:
         ldx = _rows("x", x, torch.bfloat16, self.tokens, i, self.device)
         ldl = _rows("logits", logits, torch.float32, self.tokens, self.experts, self.device)
         ldg = _rows("dout", dout, torch.bfloat16, self.tokens, o, self.device)
-        b = self._gradient_buffers()
+        self.prepare_backward()
+        b = self._grad
         h.moe_combine_backward(self.tokens, self.top_k, o, self.y, gs.R_16BF, o, rows, self.slot_row, self.row_slot,
                                self.p, dout, gs.R_16BF, ldg, b["dy"], o, b["dp"])
         h.moe_route_backward(self.tokens, self.experts, self.top_k, logits, gs.R_32F, ldl, self.ids, b["dp"],

@@ -33,7 +33,7 @@ def tensors(obj):
 def test_buffers_are_on_the_handles_device():
     """Not on the current device, which may be another by now."""
     l = layer()
-    l._gradient_buffers()
+    l.prepare_backward()
     assert {t.device for t in tensors(l)} == {torch.device("cpu")}
 
 
@@ -194,3 +194,101 @@ def test_routing_tensors_that_fit():
 def test_sizes_that_no_call_takes_are_refused(sizes):
     with pytest.raises(ValueError):
         layer(**sizes)
+
+
+def test_nothing_is_allocated_after_prepare_backward(monkeypatch):
+    l = layer()
+    l.prepare_backward()
+    buffers = [t.data_ptr() for t in tensors(l)]
+
+    def never(*args, **kw):
+        raise AssertionError("allocated")
+
+    for name in ("empty", "zeros", "empty_like", "zeros_like", "full", "tensor"):
+        monkeypatch.setattr(torch, name, never)
+    x, logits, dout = (t.clone() for t in inputs_made_before)
+    l.forward(x, logits)
+    l.backward(x, logits, dout)
+    l.prepare_backward()
+    assert buffers == [t.data_ptr() for t in tensors(l)]
+
+
+inputs_made_before = inputs()
+
+
+def test_no_buffer_is_filled():
+    """A fill would run on torch's stream, and the layer's kernels on the handle's."""
+    seen = []
+
+    class Fills(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", str(func)))
+            return func(*args, **(kwargs or {}))
+
+    with Fills():
+        layer().prepare_backward()
+    assert not [n for n in seen if "zero" in n or "fill" in n or "full" in n or "ones" in n], seen
+
+
+@pytest.mark.gpu
+def test_a_layer_made_on_another_stream_than_its_handles(cuda):
+    """Its memory was used by work that is still under way on torch's stream; the layer waits for that once."""
+    gen = torch.Generator().manual_seed(5)
+    x, logits, dout = (torch.randn(300, n, generator=gen).to(t).cuda()
+                       for n, t in ((256, torch.bfloat16), (6, torch.float32), (384, torch.bfloat16)))
+    w = torch.randn(6, 384, 256, generator=gen).cuda()
+    torch.cuda.synchronize()
+
+    def outputs(h):
+        l = layer(h, 300, 6, 2, 256, 384)
+        l.set_weights(w)
+        out = l.forward(x, logits)
+        grads = l.backward(x, logits, dout)
+        torch.cuda.synchronize()
+        assert h.device_error() == 0
+        return [t.clone() for t in (out, *grads)]
+
+    with gs.Handle() as h:
+        want = outputs(h)
+    with gs.Handle(torch.cuda.Stream()) as h:
+        for _ in range(5):
+            junk = [torch.full((3, 2 ** 20), 1e9, device="cuda") for _ in range(8)]
+            for _ in range(20):
+                for t in junk:
+                    t.mul_(1.000001)  # keeps torch's stream busy while the memory changes hands
+            del junk, t
+            for a, b in zip(want, outputs(h)):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_first_backward_under_capture(cuda):
+    """With prepare_backward, and without: the buffers are then the graph's memory."""
+    gen = torch.Generator().manual_seed(6)
+    x, logits, dout = (torch.randn(300, n, generator=gen).to(t).cuda()
+                       for n, t in ((256, torch.bfloat16), (6, torch.float32), (384, torch.bfloat16)))
+    w = torch.randn(6, 384, 256, generator=gen).cuda()
+    torch.cuda.synchronize()
+    stream, results = torch.cuda.Stream(), []
+    with gs.Handle(stream) as h:
+        for prepare in (True, False):
+            with torch.cuda.stream(stream):
+                l = layer(h, 300, 6, 2, 256, 384)
+                l.set_weights(w)
+                l.forward(x, logits)  # the kernels are loaded before the capture
+                if prepare:
+                    l.prepare_backward()
+            stream.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                l.forward(x, logits)
+                l.backward(x, logits, dout)
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert h.device_error() == 0
+            results.append([t.clone() for t in (l.out, *(l._grad[n] for n in ("dx", "dlogits", "dw")))])
+            del l, g
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
