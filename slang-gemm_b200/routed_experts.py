@@ -92,6 +92,7 @@ class RoutedExperts:
         self.y = torch.empty(rows, d_out, **bf16)  # rows behind the last expert's are neither written nor read
         self.out = torch.empty(tokens, d_out, **bf16)
         self._grad = None
+        self._ran = False
         self._settle()
 
     def _settle(self):
@@ -150,6 +151,7 @@ class RoutedExperts:
                            self.xq, gs.R_8F_E4M3, i, self.x_scale, gs.SCALE_VEC128, rows, 0.0, self.y, gs.R_16BF, o, 0)
         h.moe_combine(self.tokens, self.top_k, o, self.y, gs.R_16BF, o, rows, self.slot_row, self.p, self.out,
                       gs.R_16BF, o)
+        self._ran = True
         return self.out
 
     def backward(self, x, logits, dout):
@@ -160,6 +162,8 @@ class RoutedExperts:
         ldl = _rows("logits", logits, torch.float32, self.tokens, self.experts, self.device)
         ldg = _rows("dout", dout, torch.bfloat16, self.tokens, o, self.device)
         self.prepare_backward()
+        if not self._ran:
+            raise RuntimeError("backward without a forward: the choice and the experts' outputs are its")
         b = self._grad
         h.moe_combine_backward(self.tokens, self.top_k, o, self.y, gs.R_16BF, o, rows, self.slot_row, self.row_slot,
                                self.p, dout, gs.R_16BF, ldg, b["dy"], o, b["dp"])

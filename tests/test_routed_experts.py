@@ -196,6 +196,16 @@ def test_sizes_that_no_call_takes_are_refused(sizes):
         layer(**sizes)
 
 
+def test_backward_needs_a_forward():
+    l = layer()
+    x, logits, dout = inputs()
+    with pytest.raises(RuntimeError, match="forward"):
+        l.backward(x, logits, dout)
+    assert not l.h.calls
+    with pytest.raises(ValueError):
+        layer(align=1).backward(x, logits, dout)  # the plan can never serve one
+
+
 def test_nothing_is_allocated_after_prepare_backward(monkeypatch):
     l = layer()
     l.prepare_backward()
