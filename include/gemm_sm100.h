@@ -348,6 +348,10 @@ gs_status gs_gemm_fp8_grouped(gs_handle handle, int ragged, int transa, int tran
  * and capacity planning. */
 gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int k, int groups, int sm_count, int *columns,
                            int *ctas, int *k_slices);
+/* The same for operands of any scale modes and a C of any type; c_aligned: C, its leading dimension and its stride
+ * are multiples of 16 bytes. */
+gs_status gs_plan_gemm_fp8_ex(int ragged, int transa, int transb, int m, int n, int k, int scaleModeA, int scaleModeB,
+                              int Ctype, int c_aligned, int groups, int sm_count, int *columns, int *ctas, int *k_slices);
 
 /* ---------------------------------------------------------------------- */
 /* Routed experts around the grouped products                              */

@@ -251,11 +251,12 @@ gs_status gs_gemm_fp8(gs_handle h, int transa, int transb, int m, int n, int k, 
         [&](Context &ctx) { return launch_gemm_fp8(ctx, d); });
 }
 
-gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int k, int groups, int sm_count, int *columns,
-                           int *ctas, int *k_slices) {
+gs_status gs_plan_gemm_fp8_ex(int ragged, int transa, int transb, int m, int n, int k, int mode_a, int mode_b, int ct,
+                              int c_aligned, int groups, int sm_count, int *columns, int *ctas, int *k_slices) {
     if (!columns || !ctas || !k_slices || sm_count < 1 || m < 1 || n < 1 || k < 0 || groups < 0 || groups > GS_FP8_MAX_GROUPS)
         return GS_STATUS_INVALID_VALUE;
     if (groups > 0 && ragged != GS_GROUP_N && ragged != GS_GROUP_K) return GS_STATUS_INVALID_VALUE;
+    if (!valid_mode(mode_a) || !valid_mode(mode_b) || !float_type(ct)) return GS_STATUS_INVALID_VALUE;
     GemmFp8Desc d{};
     d.trans_a = transa != GS_OP_N;
     d.trans_b = transb != GS_OP_N;
@@ -264,13 +265,21 @@ gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int
     d.k = k;
     d.groups = groups;
     d.ragged = ragged;
-    d.b_vec = 1;
-    d.out_kind = OUT_BF16;
+    d.a_vec = mode_a == GS_SCALE_VEC128;
+    d.b_vec = mode_b == GS_SCALE_VEC128;
+    d.out_kind = ct == GS_R_32F ? OUT_F32 : ct == GS_R_16F ? OUT_F16 : OUT_BF16;
+    d.ldc = c_aligned ? 16 : 1;  // stands for any that is a multiple of 16 bytes, or is not
     const fp8::Tile t = fp8::choose_tile(d, sm_count);
     *columns = t.bn;
     *ctas = t.cg;
     *k_slices = t.split;
     return GS_STATUS_SUCCESS;
+}
+
+gs_status gs_plan_gemm_fp8(int ragged, int transa, int transb, int m, int n, int k, int groups, int sm_count, int *columns,
+                           int *ctas, int *k_slices) {
+    return gs_plan_gemm_fp8_ex(ragged, transa, transb, m, n, k, GS_SCALE_BLK128, GS_SCALE_VEC128, GS_R_16BF, 1, groups,
+                               sm_count, columns, ctas, k_slices);
 }
 
 gs_status gs_moe_rows(int tokens, int experts, int top_k, int align, int *rows) {

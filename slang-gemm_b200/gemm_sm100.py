@@ -170,6 +170,7 @@ def _load() -> ctypes.CDLL:
         "gs_gemm_fp8_grouped": (st, [vp, i, i, i, i, i, i, i, vp, vp, vp, i, i, ll, vp, i, i, ll, vp, i, i, vp, i, i, vp,
                                      vp, i, i, ll]),
         "gs_plan_gemm_fp8": (st, [i, i, i, i, i, i, i, i, ctypes.POINTER(i), ctypes.POINTER(i), ctypes.POINTER(i)]),
+        "gs_plan_gemm_fp8_ex": (st, [i] * 12 + [ctypes.POINTER(i)] * 3),
         "gs_moe_route": (st, [vp, ctypes.POINTER(RouteDesc)]),
         "gs_moe_rows": (st, [i, i, i, i, ctypes.POINTER(i)]),
         "gs_moe_route_workspace": (st, [i, i, i, ctypes.POINTER(ctypes.c_size_t)]),
@@ -330,11 +331,12 @@ def plan_tile(transa, transb, m, n, k, atype, ctype, compute, batch=1, algo=GEMM
     return s, tile.value, parts.value
 
 
-def plan_gemm_fp8(transa, transb, m, n, k, groups=0, ragged=GROUP_N, sm_count=148):
-    """gs_plan_gemm_fp8: (status, columns, ctas, k_slices) of the tile an FP8 product would use. Pure host logic."""
+def plan_gemm_fp8(transa, transb, m, n, k, groups=0, ragged=GROUP_N, sm_count=148, a_mode=SCALE_BLK128, b_mode=SCALE_VEC128,
+                  ctype=R_16BF, c_aligned=True):
+    """gs_plan_gemm_fp8_ex: (status, columns, ctas, k_slices) of the tile an FP8 product would use. Pure host logic."""
     bn, cg, parts = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
-    s = _lib.gs_plan_gemm_fp8(ragged, transa, transb, m, n, k, groups, sm_count, ctypes.byref(bn), ctypes.byref(cg),
-                              ctypes.byref(parts))
+    s = _lib.gs_plan_gemm_fp8_ex(ragged, transa, transb, m, n, k, a_mode, b_mode, ctype, int(c_aligned), groups, sm_count,
+                                 ctypes.byref(bn), ctypes.byref(cg), ctypes.byref(parts))
     return s, bn.value, cg.value, parts.value
 
 

@@ -29,7 +29,7 @@ def _check(h, call, c, want, times=4):
 @pytest.mark.parametrize("m,k,ct", [(2880, 128, BF16), (2880, 256, BF16), (2880, 256, F16), (2208, 256, F32), (2272, 256, F32)])
 def test_dense(handle, m, k, ct):
     n = 24576
-    assert gs.plan_gemm_fp8(T, N, m, n, k)[1] == 256
+    assert gs.plan_gemm_fp8(T, N, m, n, k, ctype=ct)[1] == 256
     gen = torch.Generator().manual_seed(m + k)
     a, b = Operand(gen, k, m, E4, BLK, True, True), Operand(gen, k, n, E4, VEC, True, True)
     c = torch.empty(n, m, dtype=FLOAT[ct], device="cuda")
@@ -39,11 +39,11 @@ def test_dense(handle, m, k, ct):
 
 
 @pytest.mark.parametrize("ta", [T, N])
-@pytest.mark.parametrize("m,k,ct", [(2880, 128, BF16), (2880, 256, BF16), (2208, 256, F32)])
-def test_ragged_columns(handle, ta, m, k, ct):
+@pytest.mark.parametrize("m,k,groups,ct", [(2880, 128, 32, BF16), (2880, 256, 32, BF16), (2208, 512, 8, F32)])
+def test_ragged_columns(handle, ta, m, k, groups, ct):
     """Groups that end inside a tile, and empty ones."""
-    n, groups = 24576, 32
-    assert gs.plan_gemm_fp8(ta, N, m, n, k, groups=groups)[1] == 256
+    n = 24576
+    assert gs.plan_gemm_fp8(ta, N, m, n, k, groups=groups, ctype=ct)[1] == 256
     gen = torch.Generator().manual_seed(m + k + ta)
     a = Operand(gen, k if ta else m, m if ta else k, E4, BLK, bool(ta), True, batch=groups)
     b = Operand(gen, k, n, E4, VEC, True, True)
@@ -64,6 +64,7 @@ def test_ragged_columns(handle, ta, m, k, ct):
 def test_ragged_k_with_empty_groups(handle, m, k, ma, ct):
     """Every second group is empty: its tiles write zeros right behind a tile that may still be on its way out."""
     n, groups = 2880, 16
+    assert gs.plan_gemm_fp8(N, T, m, n, k, groups=groups, ragged=gs.GROUP_K, a_mode=ma, ctype=ct)[1] == 256
     gen = torch.Generator().manual_seed(m + k)
     a, b = Operand(gen, m, k, E4, ma, False, True), Operand(gen, n, k, E4, VEC, False, True)
     step = k // (groups // 2)
