@@ -109,6 +109,7 @@ struct Args {
     long long ldc, stride_c;
     int out_kind;
     int tma_store;                     // C can be written through tmC
+    int whole_c;                       // C's rows end on 16 bytes
     int vec_c;                         // C's rows can be read and written 16 bytes at a time
     Epilogue ep;
     uint32_t *err;
@@ -686,7 +687,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < 64; ++j) acc[j] = mul2(acc[j], al);
                 }
-                if (args.tma_store && (args.ragged != GS_GROUP_N || p_warp + 32 <= it.p_end)) {
+                // A TMA store stops at the tensor's end only to the next 16 bytes: what lies behind a row that ends
+                // between them would be overwritten, so such an end is stored directly.
+                if (args.tma_store && (args.whole_c || n >= 128) && (args.ragged != GS_GROUP_N || p_warp + 32 <= it.p_end)) {
                     const int gc = args.ragged == GS_GROUP_K ? it.g : 0;
                     // `words` packs the 16 bytes of chunk x of block b
                     auto blocks = [&](auto cols_c, auto words) {
@@ -990,6 +993,7 @@ cudaError_t launch_gemm_fp8(Context &ctx, const GemmFp8Desc &d) {
     a.debug_skip_kb = ctx.debug_skip_kb;
     const size_t es = out_elem_size(d.out_kind);
     a.vec_c = aligned_c(d) ? 1 : 0;
+    a.whole_c = d.m * es % 16 == 0 ? 1 : 0;
 
     Maps maps{};
     std::string why;
