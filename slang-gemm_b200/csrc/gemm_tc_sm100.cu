@@ -40,6 +40,7 @@
 // Batches (strided or pointer-array) are the outermost tile coordinate; the
 // M/N tiles of one batch are visited in groups of `group_m` row blocks so
 // that concurrently running CTAs share A and B panels in L2.
+#include <climits>
 #include <cstdio>
 
 #include "gs_epilogue.cuh"
@@ -112,6 +113,7 @@ struct TcArgs {
                                  // fills itself from the templates tmA/tmB/tmC and args.fb's pointer arrays
     const uint32_t *c_skip_flag; // == skip_gen when a C pointer is not 16-byte aligned (C then stored directly)
     int tma_store;               // epilogue writes C with TMA tensor stores (beta == 0, C TMA-addressable)
+    int tma_rows;                // ... in warps whose 32 rows end at or before this one
     int ab_evict_last;           // operand loads use the evict_last L2 policy
     simt::SimtArgs fb;           // pointer-array batches: the CUDA-core fallback's view of the problem
     Epilogue ep;
@@ -490,6 +492,7 @@ __global__ void __launch_bounds__(Cfg<CG, WIDE>::THREADS, 1)
             int b, mb, nb;
             tile_coords(args, t, b, mb, nb);
             const int m = mb * C_::TILE_M + static_cast<int>(rank) * BM + row;
+            const bool warp_tma = c_tma && m - lane <= args.tma_rows - 32;
             const int nfills = chunked ? (args.k_blocks + CHUNK_KB - 1) / CHUNK_KB : 1;
             if constexpr (CHUNKED) {
                 // Fold every fill but the last into the running sum (columns BN..2BN-1), in order.
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(Cfg<CG, WIDE>::THREADS, 1)
                 } else {
                     tmem_wait_ld();
                 }
-                if (c_tma) {
+                if (warp_tma) {
                     // Stage this warp's 32 rows in blocks of 16 columns (column-major, like C)
                     // and write each block with one TMA tensor store; edge elements are
                     // clipped by TMA. Two staging buffers per warp alternate.
@@ -825,6 +828,9 @@ static TcArgs make_args(Context &ctx, const GemmDesc &d, int shape) {
     a.C = d.C;
     a.ldc = d.ldc;
     a.stride_c = d.stride_c;
+    // A TMA store stops at the tensor's end only to the next 16 bytes: a column of C that ends between them has its last
+    // rows stored directly, so that what lies behind them stays.
+    a.tma_rows = static_cast<uint64_t>(d.m) * out_elem_size(d.out_kind) % 16 == 0 ? INT_MAX : d.m;
     a.c_arr = nullptr;
     a.a_maps = nullptr;
     a.b_maps = nullptr;
