@@ -269,7 +269,8 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
                     record(a1, a2, g);
                 }
             }
-            const Key mine = k1 == none ? none : key_of(value_of(k1) + (k2 != none ? value_of(k2) : R(0)));
+            const R c1 = value_of(k1), c2 = k2 != none ? value_of(k2) : R(0);
+            const Key mine = k1 == none ? none : key_of(c1 + c2);
             int better = 0;
             for (int g = 0; g < d.groups; ++g) {
                 const Key other = __shfl_sync(kFull, mine, g);
@@ -277,12 +278,12 @@ __device__ __forceinline__ bool choose(const RouteDesc &d, const float (&l)[VPL]
             }
             const bool kept = lane < d.groups && better < d.top_groups;
             if constexpr (F32) {
-                // How far the sum may be off: each of its two c by its own size, however small their sum, and the steps
-                // of the sum and of its limit. The least that a kept group may have has to pass the most that another may.
-                // A sum beyond f32's range may be anything (its limits are NaN, or infinite).
+                // How far the sum may be off: by its two terms' scores, and by half a step (6e-8 of it) of each c, of the
+                // sum and of its limit, none of them larger than |c1| + |c2|, however small the sum is. The least that a
+                // kept group may have has to pass the most that another may. A sum beyond f32's range may be anything
+                // (its limits are NaN, or infinite).
                 const bool live = k1 != none;
-                const float sum = value_of(mine);
-                const float reach = live ? doubt(d, value_of(k1)) + (k2 != none ? doubt(d, value_of(k2)) : 0.0f) + 2e-7f * fabsf(sum) : 0.0f;
+                const float sum = c1 + c2, reach = 2.0f * doubt(d, 0.0f) + 2e-7f * (fabsf(c1) + fabsf(c2));
                 const Key worst = ~warp_max(kept && live ? ~key_of(fmaxf(sum - reach, -INFINITY)) : Key(0));
                 const Key best = warp_max(!kept && live ? key_of(fminf(sum + reach, INFINITY)) : Key(0));
                 if (best >= worst) close = true;
