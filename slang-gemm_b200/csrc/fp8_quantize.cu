@@ -18,7 +18,7 @@
 // registers between the maximum and the cast. 8192 x 8192 f32 in blocks: 51 us, 6.5
 // TB/s. Vectors of bf16 come near it (4096 x 16384: 36 us, 5.6 TB/s) and, gathered from
 // a source that fits L2, are bound by instruction issue (31 us). Vectors along the
-// rows cross threads: 73 us, 2.8 TB/s.
+// rows cross threads and three barriers a tile: 72 us, 2.8 TB/s (f32: 87 us, 3.9).
 #include <cuda_fp8.h>
 
 #include <cstring>

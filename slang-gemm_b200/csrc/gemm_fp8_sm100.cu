@@ -44,10 +44,13 @@
 //
 // Bounds. Wide tiles: the promoters and the two slots' handshake, 776 cycles a K
 // block with a scale per row and block, 1358 with one per row and column, for 512
-// of tensor core; 8192^3 to bf16 takes 486 us (2260 TFLOP/s) cool and 578 under the
-// power cap. Narrow tiles: reading A; 64 groups of 2048 x 2048 with two rows each on
-// average take 35 us (7.5 TB/s counting empty groups), 4096 x 16 x 4096 7.2 us, of which
-// 2.6 would be the bytes and the rest is launch, first loads and the reduction.
+// of tensor core, and about 4000 cycles a tile in which the promoters store C and
+// the tensor core waits; 8192^3 to bf16 takes 561 to 577 us in repeated calls (1910
+// to 1960 TFLOP/s; the clock falls to 1.5 GHz), 480 to 490 in a short run. Narrow
+// tiles: reading A; 64 groups of 2048 x 2048 with two rows each on average, 44 of
+// them not empty, take 39 to 41 us (185 MB, 4.6 TB/s; 704 tiles on 148 SMs are 4.8
+// rounds), 4096 x 16 x 4096 7.2 us, of which 2.6 would be the bytes and the rest is
+// launch, first loads and the reduction.
 #include <type_traits>
 
 #include "gs_epilogue.cuh"

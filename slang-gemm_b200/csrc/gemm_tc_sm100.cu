@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(Cfg<CG, WIDE>::THREADS, 1)
                 }
                 if (warp_tma) {
                     // Stage this warp's 32 rows in blocks of 16 columns (column-major, like C)
-                    // and write each block with one TMA tensor store; edge elements are
-                    // clipped by TMA. Two staging buffers per warp alternate.
+                    // and write each block with one TMA tensor store, which leaves out what lies outside C (see
+                    // tma_rows). Two staging buffers per warp alternate.
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (c + 16 * h >= ncols) continue;

@@ -21,9 +21,15 @@
 // launch.
 //
 // Bound by instruction issue (about 1400 a token at 256 experts in 8 groups with a
-// bias and top_k 8, 600 without groups and bias): 16384 tokens take 48 us, 33 of
-// them the choice; 48 tokens of 64 experts take 9 us, the latency of one block. The
-// gradient of 16383 x 160 softmax logits takes 11 us.
+// bias and top_k 8, 600 without groups and bias): 16384 tokens take 47 to 51 us, 35
+// of them the choice. 48 tokens of 64 experts take 9 us: one block, three tokens a
+// warp one after another (the choice alone 6.5 us), then the plan. The gradient of
+// 16383 x 160 softmax logits takes 11 us.
+//
+// Meant for up to 256 experts. Above, a lane holds 16 or 32 logits and the choice
+// spills (its f64 form most): 16384 tokens, top_k 8, take 45 us at 512
+// experts and 57 at 1024, with groups and a bias 103 and 150; 48 tokens 24 and 34 us;
+// the softmax gradient of 16384 tokens 24 and 55 us.
 #include <atomic>
 #include <type_traits>
 
