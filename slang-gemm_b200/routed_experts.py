@@ -33,9 +33,13 @@ def _blocks(n: int) -> int:
 
 
 def _rows(name, t, dtype, rows, cols, device):
-    """The leading dimension of t, a rows x cols matrix as the kernels read it; ValueError if it is another. Looks at no
-    value, so it may run under capture."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows, cols) or t.device != device:
+    """The leading dimension of t, a rows x cols matrix as the kernels read it (or a contiguous [..., cols] of as many rows);
+    ValueError if it is another. Looks at no value, so it may run under capture."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] on {device}, not {_describe(t)}")
+    if t.shape != (rows, cols):
+        if t.dim() > 2 and t.shape[-1] == cols and t.numel() == rows * cols and t.is_contiguous():
+            return cols
         raise ValueError(f"{name} must be {dtype} [{rows}, {cols}] on {device}, not {_describe(t)}")
     ld, step = t.stride()
     if (step != 1 and cols > 1) or (ld < cols and rows > 1):
@@ -47,11 +51,11 @@ def _describe(t) -> str:
     return f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
 
 
-def _vector(name, t, dtype, shapes, device):
-    """ValueError unless t is None or contiguous, of one of `shapes`."""
-    if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) in shapes and
-                              t.device == device and t.is_contiguous()):
-        raise ValueError(f"{name} must be {dtype} {list(shapes[0])} on {device}, contiguous, not {_describe(t)}")
+def _vector(name, t, dtype, n, device):
+    """ValueError unless t is None or n contiguous elements."""
+    if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.numel() == n and t.device == device and
+                              t.is_contiguous()):
+        raise ValueError(f"{name} must be {dtype} [{n}] on {device}, contiguous, not {_describe(t)}")
 
 
 class RoutedExperts:
@@ -71,8 +75,8 @@ class RoutedExperts:
                             scale=scale, token_count=token_count)
         self.rows = rows = gs.moe_rows(tokens, experts, top_k, align)
         self.device = torch.device(handle.device)
-        _vector("bias", bias, torch.float32, [(experts,)], self.device)
-        _vector("token_count", token_count, torch.int32, [(1,), ()], self.device)
+        _vector("bias", bias, torch.float32, experts, self.device)
+        _vector("token_count", token_count, torch.int32, 1, self.device)
         i32, u8, f32, bf16 = (dict(dtype=t, device=self.device)
                               for t in (torch.int32, torch.uint8, torch.float32, torch.bfloat16))
         self.ids, self.p = torch.empty(tokens, top_k, **i32), torch.empty(tokens, top_k, **f32)

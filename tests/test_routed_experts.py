@@ -97,6 +97,17 @@ def test_rows_may_lie_apart():
     assert args[10] is wide[2] and args[12] == 56
 
 
+def test_rows_may_have_more_than_one_axis():
+    """[batch, sequence, features] without a gap is as many rows."""
+    l = layer(tokens=6)
+    x, logits, dout = (t.view(2, 3, -1) for t in inputs(6))
+    l.forward(x, logits)
+    l.backward(x, logits, dout)
+    assert [args[5] for name, args, _ in l.h.calls if name == "moe_route"] == [4]
+    with pytest.raises(ValueError, match="x"):
+        l.forward(torch.cat([x, x], 2)[..., :32], logits)
+
+
 def test_one_token_may_have_any_row_stride():
     l = layer(tokens=1)
     x, logits, dout = (torch.as_strided(t, t.shape, (1, 1)) for t in inputs(1))
@@ -175,7 +186,7 @@ def test_weights_can_be_shared_by_layers_of_other_batches():
 
 @pytest.mark.parametrize("name,value", [
     ("bias", torch.zeros(5)), ("bias", torch.zeros(4, dtype=torch.bfloat16)), ("bias", torch.zeros(8)[::2]),
-    ("bias", torch.zeros(4, 1)), ("bias", torch.zeros(4, device="meta")), ("bias", [0.0] * 4),
+    ("bias", torch.zeros(4, 2)), ("bias", torch.zeros(4, device="meta")), ("bias", [0.0] * 4),
     ("token_count", torch.tensor([3])), ("token_count", torch.tensor([3.0])), ("token_count", torch.tensor([], dtype=torch.int32)),
     ("token_count", torch.tensor([3, 4], dtype=torch.int32)), ("token_count", torch.tensor([3], dtype=torch.int32, device="meta")),
     ("token_count", 3),
@@ -187,7 +198,7 @@ def test_routing_tensors_that_would_be_read_wrongly_are_refused(name, value):
 
 def test_routing_tensors_that_fit():
     layer(bias=torch.zeros(4), token_count=torch.tensor([3], dtype=torch.int32))
-    layer(token_count=torch.tensor(3, dtype=torch.int32))
+    layer(bias=torch.zeros(1, 4), token_count=torch.tensor(3, dtype=torch.int32))
 
 
 @pytest.mark.parametrize("sizes", [dict(tokens=0), dict(tokens=-1), dict(d_in=0), dict(d_out=-16), dict(d_in=24), dict(d_out=40)])
